@@ -99,6 +99,11 @@ SIGNATURES = {
     "kda_cast_weights_bf16": (ctypes.c_int, [_I, ctypes.POINTER(ctypes.c_void_p), ctypes.POINTER(ctypes.c_int64), _P, _P]),
     "kda_chunk_forward_conv_norm_gate_infer": (ctypes.c_int, [_PP, _P, _L, _P, _I] + [_P] * 10 + [_F] + [_P] * 4),
     "kda_embedding_backward": (ctypes.c_int, [_L, _I, _I, _P, _P, _P, _P]),
+    "kda_softcap_log_probs_forward": (ctypes.c_int, [_L, _I, _L, _F, _P, _P, _L] + [_P] * 5),
+    "kda_softcap_log_probs_backward": (ctypes.c_int, [_L, _I, _L, _F, _P, _P, _L] + [_P] * 7),
+    "kda_policy_rows": (ctypes.c_int, [_L, _P, _L, _P, _P, _P, _P, _P, _F, _F, _F, _P, _P, _P, _P]),
+    "kda_preference_pairs_scratch_bytes": (ctypes.c_size_t, [_I]),
+    "kda_preference_pairs": (ctypes.c_int, [_L, _L, _I, _P, _P, _L, _P, _P, _F, _F, _I] + [_P] * 6),
 }
 
 _lib = None

@@ -17,10 +17,12 @@ from __future__ import annotations
 import math
 import os
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import ops
 from .kda import KDAState, KimiDeltaAttention, Linear, linear_few_rows, plain
@@ -190,6 +192,218 @@ def softcap_cross_entropy(logits, targets, vocab, softcap=15.0, ignore_index=-1,
         return _SoftcapCrossEntropy.apply(logits, targets, vocab, float(softcap), ignore_index)
     z = softcap * torch.tanh(logits[:, :vocab].float() / softcap)
     return F.cross_entropy(z, targets, ignore_index=ignore_index)
+
+
+class _SoftcapLogProbs(torch.autograd.Function):
+    """Row log-probabilities (and entropies) on the HIP kernels: one read of the bf16 logits
+    forward, one read and one write of the bf16 logit gradient backward."""
+
+    @staticmethod
+    def forward(ctx, logits, targets, vocab, softcap, ignore_index, entropy):
+        logp, lse, ent = ops.softcap_log_probs_forward(logits, targets, vocab, softcap, ignore_index, entropy=entropy)
+        ctx.save_for_backward(logits, targets, lse, ent)
+        ctx.args = (vocab, softcap, ignore_index)
+        ctx.set_materialize_grads(False)
+        return logp, ent
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, h):
+        logits, targets, lse, ent = ctx.saved_tensors
+        if g is None and h is None:
+            return (None,) * 6
+        return (ops.softcap_log_probs_backward(logits, targets, lse, ent, g, h, *ctx.args), *(None,) * 5)
+
+
+class _PolicyLoss(torch.autograd.Function):
+    """The clipped policy loss on the HIP kernels: the log-probability pass, one kernel over the
+    rows that leaves every row's slope, and the logit gradient for those slopes."""
+
+    @staticmethod
+    def forward(ctx, logits, targets, old, adv, ref, weights, vocab, softcap, ignore_index, lo, hi, kl_coef, grad):
+        logp, lse, _ = ops.softcap_log_probs_forward(logits, targets, vocab, softcap, ignore_index)
+        loss, stats, slope = ops.policy_rows(targets, logp, old, adv, ref, weights, lo, hi, kl_coef, ignore_index,
+                                             slopes=grad)
+        ctx.save_for_backward(logits, targets, lse, slope)
+        ctx.args = (vocab, softcap, ignore_index)
+        ctx.mark_non_differentiable(logp, stats)
+        return loss, logp, stats
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad, _logp, _stats):
+        logits, targets, lse, slope = ctx.saved_tensors
+        return (ops.softcap_log_probs_backward(logits, targets, lse, None, slope, None, *ctx.args, scale=grad),
+                *(None,) * 12)
+
+
+class _PreferenceLoss(torch.autograd.Function):
+    """The preference loss on the HIP kernels: the log-probability pass, one kernel over sequences
+    and pairs that leaves every row's slope, and the logit gradient for those slopes."""
+
+    @staticmethod
+    def forward(ctx, logits, targets, pairs, seq_len, cu_seqlens, ref, vocab, softcap, ignore_index, beta, smoothing,
+                average, grad):
+        logp, lse, _ = ops.softcap_log_probs_forward(logits, targets, vocab, softcap, ignore_index, double=True)
+        loss, seq, margins, slope = ops.preference_pairs(targets, logp, pairs, seq_len, cu_seqlens, ref, beta,
+                                                         smoothing, average, ignore_index, slopes=grad)
+        ctx.save_for_backward(logits, targets, lse, slope)
+        ctx.args = (vocab, softcap, ignore_index)
+        ctx.mark_non_differentiable(seq, margins)
+        return loss, seq, margins
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad, _seq, _margins):
+        logits, targets, lse, slope = ctx.saved_tensors
+        return (ops.softcap_log_probs_backward(logits, targets, lse, None, slope, None, *ctx.args, scale=grad),
+                *(None,) * 12)
+
+
+def _flat_tokens(what, logits, targets, vocab, *rows):
+    """(logits [rows, columns], targets [rows], row tensors [rows] in f32) of [..., columns] logits
+    and tensors of the leading shape."""
+    if logits.ndim < 1 or targets.shape != logits.shape[:-1] or any(t is not None and t.shape != targets.shape for t in rows):
+        raise ValueError(f"{what}: logits [..., columns] and one target and row value for each leading position expected")
+    if not 0 < vocab <= logits.shape[-1]:
+        raise ValueError(f"{what}: vocab must be in [1, {logits.shape[-1]}]")
+    return (logits.reshape(-1, logits.shape[-1]), targets.reshape(-1),
+            *(None if t is None else t.detach().reshape(-1).float() for t in rows))
+
+
+def _eager_log_probs(logits, targets, vocab, softcap, ignore_index):
+    """(log-probabilities, entropies) of 2-D logits of any type and device, in f32 or more."""
+    wide = torch.float64 if logits.dtype == torch.float64 else torch.float32
+    keep = targets != ignore_index
+    z = softcap * torch.tanh(torch.where(keep[:, None], logits[:, :vocab].to(wide), 0.0) / softcap)
+    q = torch.log_softmax(z, -1)
+    bad = (targets < 0) | (targets >= vocab)
+    logp = q.gather(1, targets.masked_fill(bad, 0)[:, None])[:, 0].masked_fill(bad, float("nan"))
+    return torch.where(keep, logp, 0.0), torch.where(keep, -(q.exp() * q).sum(-1), 0.0)
+
+
+def softcap_log_probs(logits, targets, vocab, softcap=15.0, ignore_index=-1, *, entropy=False):
+    """log softmax(softcap * tanh(logits[..., :vocab] / softcap)) at ``targets``: f32, shaped like
+    targets; with ``entropy`` (log-probabilities, entropies of the softmax).  Rows whose target is
+    ignore_index give 0 and are not read.  Differentiable by the logits (bf16 CUDA logits run the
+    HIP kernels, anything else the eager f32 form), once."""
+    flat, t = _flat_tokens("softcap_log_probs", logits, targets, vocab)
+    if logits.is_cuda and logits.dtype == torch.bfloat16:
+        logp, ent = _SoftcapLogProbs.apply(flat, t, vocab, float(softcap), ignore_index, entropy)
+    else:
+        logp, ent = _eager_log_probs(flat, t, vocab, softcap, ignore_index)
+    return (logp.view(targets.shape), ent.view(targets.shape)) if entropy else logp.view(targets.shape)
+
+
+class PolicyLoss(NamedTuple):
+    """``loss`` is differentiable; the others are for the log: the rows' log-probabilities (the next
+    ``old_log_probs``), the KL estimate and the share of the weight whose ratio was clipped."""
+
+    loss: torch.Tensor
+    log_probs: torch.Tensor
+    kl: torch.Tensor
+    clip_fraction: torch.Tensor
+
+
+def policy_loss(logits, targets, old_log_probs, advantages, vocab, softcap=15.0, ignore_index=-1, *,
+                ref_log_probs=None, clip=0.2, clip_high=None, kl_coef=0.0, weights=None):
+    """Clipped policy loss over the tokens ``targets`` of sampled sequences, with soft-capped
+    logits [..., columns]:
+
+      sum_r w_r (-min(q_r A_r, clamp(q_r, 1 - clip, 1 + clip_high) A_r) + kl_coef (e^d_r - d_r - 1)),
+
+    q = exp(logp - old_log_probs), d = ref_log_probs - logp (no KL term without ref_log_probs), w =
+    ``weights`` or, by default, the mean over the rows whose target is not ignore_index (NaN if
+    there is none, as the cross entropy's).  Rows without a target or of weight 0 are not counted (their
+    log_probs are 0).
+    clip_high defaults to clip.  The row tensors are shaped like targets and are constants.
+    Returns a PolicyLoss."""
+    flat, t, old, adv, ref, w = _flat_tokens("policy_loss", logits, targets, vocab, old_log_probs, advantages,
+                                             ref_log_probs, weights)
+    clip_high = clip if clip_high is None else clip_high
+    if not (0.0 <= clip <= 1.0 and clip_high >= 0.0):
+        raise ValueError("policy_loss: clip must be in [0, 1] and clip_high not negative")
+    lo, hi = 1.0 - clip, 1.0 + clip_high
+    if logits.is_cuda and logits.dtype == torch.bfloat16:
+        if w is not None:  # rows of weight 0 need not be read
+            t = torch.where(w != 0, t, ignore_index)
+        loss, logp, stats = _PolicyLoss.apply(flat, t, old, adv, ref, w, vocab, float(softcap), ignore_index, lo, hi,
+                                              float(kl_coef), torch.is_grad_enabled() and logits.requires_grad)
+        return PolicyLoss(loss, logp.view(targets.shape), stats[0], stats[1])
+    if w is not None:
+        t = torch.where(w != 0, t, ignore_index)
+    keep = t != ignore_index
+    logp, _ = _eager_log_probs(flat, t, vocab, softcap, ignore_index)
+    w = keep.to(logp.dtype) / keep.sum() if w is None else w
+    old, adv, w = (torch.where(keep, v.to(logp.dtype), 0.0) for v in (old, adv, w))
+    ratio = (logp - old).exp()
+    free = torch.where(adv == 0, 0.0, ratio * adv)
+    held = ratio.clamp(lo, hi) * adv
+    clipped = held < free
+    rows, kl = -torch.where(clipped, held, free), torch.zeros_like(w)
+    if ref is not None:
+        d = torch.where(keep, ref.to(logp.dtype) - logp, 0.0)
+        kl = torch.expm1(d) - d
+        rows = rows + kl_coef * kl if kl_coef else rows
+    return PolicyLoss((w * rows).sum(), logp.detach().view(targets.shape), (w * kl).sum().detach(),
+                      (w * clipped).sum().detach())
+
+
+class PreferenceLoss(NamedTuple):
+    """``loss`` is differentiable; ``log_probs`` [2 P] are the sequences' log-probabilities (under the
+    reference they are the ``ref_log_probs``), ``margins`` [P] the implicit rewards' differences
+    (positive: the pair is ordered rightly)."""
+
+    loss: torch.Tensor
+    log_probs: torch.Tensor
+    margins: torch.Tensor
+
+
+def preference_loss(logits, targets, vocab, softcap=15.0, ignore_index=-1, *, beta=0.1, ref_log_probs=None,
+                    label_smoothing=0.0, average=False, cu_seqlens=None):
+    """Preference loss of P pairs of sequences under soft-capped logits: with s the summed (average:
+    mean) log-probability of a sequence's tokens whose target is not ignore_index,
+
+      m = beta ((s_chosen - ref_chosen) - (s_rejected - ref_rejected))
+      loss = mean over pairs of -(1 - label_smoothing) log sigmoid(m) - label_smoothing log sigmoid(-m).
+
+    Sequences are the rows of logits [2 P, T, columns] and targets [2 P, T], the P chosen ones first
+    and their rejected partners after them in the same order; or packed, logits [rows, columns] and
+    targets [rows] with ``cu_seqlens`` [2 P + 1] int32 (non-decreasing, within the rows: the kernels
+    make everything NaN otherwise).  ``ref_log_probs`` [2 P] f32: the sequences' log-probabilities
+    under the reference (None: zeros).  Returns a PreferenceLoss."""
+    if cu_seqlens is None:
+        if logits.ndim != 3:
+            raise ValueError("preference_loss: logits [2 P, T, columns] expected without cu_seqlens")
+        n, seq_len = logits.shape[0], logits.shape[1]
+    else:
+        if logits.ndim != 2 or cu_seqlens.ndim != 1 or cu_seqlens.dtype != torch.int32:
+            raise ValueError("preference_loss: packed logits [rows, columns] and cu_seqlens int32 [2 P + 1] expected")
+        n, seq_len = cu_seqlens.numel() - 1, 0
+    if n <= 0 or n % 2:
+        raise ValueError("preference_loss: an even number of sequences expected, chosen and rejected")
+    if ref_log_probs is not None and ref_log_probs.shape != (n,):
+        raise ValueError(f"preference_loss: ref_log_probs must have shape {(n,)}")
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError("preference_loss: label_smoothing must be in [0, 1]")
+    flat, t = _flat_tokens("preference_loss", logits, targets, vocab)
+    ref = None if ref_log_probs is None else ref_log_probs.detach().float()
+    if logits.is_cuda and logits.dtype == torch.bfloat16:
+        return PreferenceLoss(*_PreferenceLoss.apply(
+            flat, t, n // 2, seq_len, cu_seqlens, ref, vocab, float(softcap), ignore_index, float(beta),
+            float(label_smoothing), bool(average), torch.is_grad_enabled() and logits.requires_grad))
+    logp, _ = _eager_log_probs(flat, t, vocab, softcap, ignore_index)
+    keep = t != ignore_index
+    at = list(range(0, flat.shape[0] + 1, seq_len)) if cu_seqlens is None and seq_len else \
+        [0] * (n + 1) if cu_seqlens is None else cu_seqlens.tolist()
+    if at[0] < 0 or at[-1] > flat.shape[0] or any(a > b for a, b in zip(at, at[1:])):
+        raise ValueError("preference_loss: cu_seqlens must be non-decreasing and within the rows")
+    s = torch.stack([logp[a:b].double().sum() / (keep[a:b].sum().clamp(min=1) if average else 1)
+                     for a, b in zip(at, at[1:])])
+    gain = s if ref is None else s - ref
+    m = beta * (gain[:n // 2] - gain[n // 2:])
+    loss = -((1 - label_smoothing) * F.logsigmoid(m) + label_smoothing * F.logsigmoid(-m)).mean()
+    return PreferenceLoss(loss.to(logp.dtype), s.detach().to(logp.dtype), m.detach().to(logp.dtype))
 
 
 class _Relu2(torch.autograd.Function):
@@ -543,6 +757,29 @@ class GPT(nn.Module):
         all-KDA model: no rotary tables or value embeddings).  With a cache, a prompt
         prefill (T > 1) smears within the prompt only, and a one-token step smears with the
         cached previous embedding."""
+        logits = self._logits(idx, kv_cache)
+        if targets is not None:
+            return softcap_cross_entropy(logits.flatten(0, 1), targets.flatten(), self.config.vocab_size,
+                                         15.0, -1, expected_grad=self.loss_grad_hint)
+        return 15 * torch.tanh(logits[..., : self.config.vocab_size].float() / 15)
+
+    def token_log_probs(self, idx, targets, *, entropy=False):
+        """``softcap_log_probs`` of ``targets`` [B, T] (-1: none) after the tokens ``idx`` [B, T]."""
+        return softcap_log_probs(self._logits(idx), targets, self.config.vocab_size, 15.0, -1, entropy=entropy)
+
+    def policy_loss(self, idx, targets, old_log_probs, advantages, **options):
+        """``policy_loss`` of sampled sequences: ``targets`` [B, T] (-1: none, as in a prompt) after
+        the tokens ``idx`` [B, T], and the row tensors [B, T]."""
+        return policy_loss(self._logits(idx), targets, old_log_probs, advantages, self.config.vocab_size, 15.0, -1,
+                           **options)
+
+    def preference_loss(self, idx, targets, **options):
+        """``preference_loss`` of the sequences ``idx`` [2 P, T] (chosen ones first) and their
+        ``targets`` [2 P, T] (-1: none, as in a prompt or padding)."""
+        return preference_loss(self._logits(idx), targets, self.config.vocab_size, 15.0, -1, **options)
+
+    def _logits(self, idx, kv_cache=None):
+        """The lm_head's output [B, T, padded vocabulary] before the soft cap."""
         n_tok = idx.shape[1]
         x = norm(embed(self.transformer.wte, idx).to(torch.bfloat16))
         before = None
@@ -567,11 +804,7 @@ class GPT(nn.Module):
             if mid_out is not None:
                 x = resid_mix(x, mid_out, self._one, -self.backout_lambda, 0)
             h = norm(x)
-        logits = self.lm_head(h)
-        if targets is not None:
-            return softcap_cross_entropy(logits.flatten(0, 1), targets.flatten(), self.config.vocab_size,
-                                         15.0, -1, expected_grad=self.loss_grad_hint)
-        return 15 * torch.tanh(logits[..., : self.config.vocab_size].float() / 15)
+        return self.lm_head(h)
 
 
 GEMM_SELECTION_FILE = os.path.join(os.path.dirname(os.path.abspath(__file__)), "gemm_selection_gfx950.csv")

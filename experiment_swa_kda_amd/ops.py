@@ -823,6 +823,120 @@ def softcap_cross_entropy_backward(logits, targets, lse, grad_scale, vocab, soft
     check(rc, "kda_softcap_cross_entropy_backward")
     return grad
 
+
+def _token_inputs(what, logits, targets, *rows):
+    """Checks logits [rows, stride], targets [rows] and f32 row tensors [rows] (or None)."""
+    dev = _require_cuda(what, logits, targets, *rows)
+    _check_dtype(what, logits, torch.bfloat16, "logits")
+    _check_dtype(what, targets, torch.int64, "targets")
+    if logits.ndim != 2 or targets.shape != logits.shape[:1]:
+        raise RuntimeError(f"{what}: logits [rows, stride] and targets [rows]")
+    _check_rows(what, targets, *rows)
+    return dev
+
+
+def _check_rows(what, targets, *rows):
+    for t in rows:
+        _check_dtype(what, t, torch.float32, "row values")
+        if t is not None and t.shape != targets.shape:
+            raise RuntimeError(f"{what}: one row value for each target expected")
+
+
+def softcap_log_probs_forward(logits, targets, vocab, softcap, ignore_index=-1, *, entropy=False, double=False):
+    """logits [rows, stride] bf16 (stride >= vocab), targets [rows] int64 -> (log-probabilities f32
+    [rows], with ``double`` f64, lse f32 [rows], entropies f32 [rows] or None); zeros in the rows
+    whose target is ignore_index, which are not read."""
+    what = "softcap_log_probs_forward"
+    dev = _token_inputs(what, logits, targets)
+    logits, targets = _c(logits), _c(targets)
+    rows, stride = logits.shape
+    logp = torch.empty(rows, dtype=torch.float64 if double else torch.float32, device=dev)
+    lse = torch.empty(rows, dtype=torch.float32, device=dev)
+    ent = torch.empty(rows, dtype=torch.float32, device=dev) if entropy else None
+    with _on(dev):
+        rc = _lib.load().kda_softcap_log_probs_forward(
+            rows, int(vocab), stride, float(softcap), ptr(logits), ptr(targets), int(ignore_index),
+            None if double else ptr(logp), ptr(logp) if double else None, ptr(lse), ptr(ent), _stream(dev))
+    check(rc, "kda_softcap_log_probs_forward")
+    return logp, lse, ent
+
+
+def softcap_log_probs_backward(logits, targets, lse, entropy, g, h, vocab, softcap, ignore_index=-1, *, scale=None):
+    """Logit gradient [rows, stride] bf16 for row gradients ``g`` of the log-probabilities and ``h``
+    of the entropies (f32 [rows], either None), both times the one-element tensor ``scale``."""
+    what = "softcap_log_probs_backward"
+    dev = _token_inputs(what, logits, targets, lse, entropy, g, h)
+    if g is None and h is None or h is not None and entropy is None:
+        raise RuntimeError(f"{what}: a row gradient is needed, and for the entropies' the entropies")
+    logits, targets, lse, entropy, g, h = (_c(t) for t in (logits, targets, lse, entropy, g, h))
+    if scale is not None:
+        scale = scale.to(device=dev, dtype=torch.float32).reshape(1).contiguous()
+    rows, stride = logits.shape
+    grad = torch.empty_like(logits)
+    with _on(dev):
+        rc = _lib.load().kda_softcap_log_probs_backward(
+            rows, int(vocab), stride, float(softcap), ptr(logits), ptr(targets), int(ignore_index), ptr(lse),
+            ptr(entropy), ptr(g), ptr(h), ptr(scale), ptr(grad), _stream(dev))
+    check(rc, "kda_softcap_log_probs_backward")
+    return grad
+
+
+def policy_rows(targets, log_probs, old_log_probs, advantages, ref_log_probs, weights, clip_lo, clip_hi, kl_coef,
+                ignore_index=-1, *, slopes=False):
+    """Clipped policy loss of f32 row log-probabilities -> (loss, stats [2] = (KL, weight of the
+    clipped rows), d loss / d log_probs [rows] or None)."""
+    what = "policy_rows"
+    dev = _require_cuda(what, targets, log_probs, old_log_probs, advantages, ref_log_probs, weights)
+    _check_dtype(what, targets, torch.int64, "targets")
+    if targets.ndim != 1 or old_log_probs is None or advantages is None:
+        raise RuntimeError(f"{what}: targets, log_probs, old_log_probs and advantages [rows] expected")
+    _check_rows(what, targets, log_probs, old_log_probs, advantages, ref_log_probs, weights)
+    targets, log_probs, old_log_probs, advantages, ref_log_probs, weights = (
+        _c(t) for t in (targets, log_probs, old_log_probs, advantages, ref_log_probs, weights))
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    stats = torch.empty(2, dtype=torch.float32, device=dev)
+    slope = torch.empty_like(log_probs) if slopes else None
+    with _on(dev):
+        rc = _lib.load().kda_policy_rows(
+            targets.numel(), ptr(targets), int(ignore_index), ptr(log_probs), ptr(old_log_probs), ptr(advantages),
+            ptr(ref_log_probs), ptr(weights), float(clip_lo), float(clip_hi), float(kl_coef), ptr(loss), ptr(stats),
+            ptr(slope), _stream(dev))
+    check(rc, "kda_policy_rows")
+    return loss, stats, slope
+
+
+def preference_pairs(targets, log_probs64, pairs, seq_len, cu_seqlens, ref_log_probs, beta, label_smoothing, average,
+                     ignore_index=-1, *, slopes=False):
+    """Preference loss of f64 row log-probabilities [rows] -> (loss, sequence log-probabilities
+    [2 pairs], margins [pairs], d loss / d row log-probability [rows] or None)."""
+    what = "preference_pairs"
+    dev = _require_cuda(what, targets, log_probs64, cu_seqlens, ref_log_probs)
+    _check_dtype(what, targets, torch.int64, "targets")
+    _check_dtype(what, log_probs64, torch.float64, "log_probs64")
+    _check_dtype(what, cu_seqlens, torch.int32, "cu_seqlens")
+    _check_dtype(what, ref_log_probs, torch.float32, "ref_log_probs")
+    if targets.ndim != 1 or log_probs64.shape != targets.shape:
+        raise RuntimeError(f"{what}: targets and log_probs64 [rows] expected")
+    if cu_seqlens is not None and cu_seqlens.shape != (2 * pairs + 1,):
+        raise RuntimeError(f"{what}: cu_seqlens must have 2 pairs + 1 entries")
+    if ref_log_probs is not None and ref_log_probs.shape != (2 * pairs,):
+        raise RuntimeError(f"{what}: ref_log_probs must have 2 pairs entries")
+    targets, log_probs64, cu_seqlens, ref_log_probs = (_c(t) for t in (targets, log_probs64, cu_seqlens, ref_log_probs))
+    lib = _lib.load()
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    seq = torch.empty(2 * pairs, dtype=torch.float32, device=dev)
+    margins = torch.empty(pairs, dtype=torch.float32, device=dev)
+    slope = torch.empty(targets.numel(), dtype=torch.float32, device=dev) if slopes else None
+    scratch = torch.empty(lib.kda_preference_pairs_scratch_bytes(pairs), dtype=torch.uint8, device=dev)
+    with _on(dev):
+        rc = lib.kda_preference_pairs(
+            targets.numel(), int(seq_len), int(pairs), ptr(cu_seqlens), ptr(targets), int(ignore_index),
+            ptr(log_probs64), ptr(ref_log_probs), float(beta), float(label_smoothing), 1 if average else 0, ptr(loss),
+            ptr(seq), ptr(margins), ptr(slope), ptr(scratch), _stream(dev))
+    check(rc, "kda_preference_pairs")
+    return loss, seq, margins, slope
+
+
 def weight_grad(grad_output, x):
     """dW [N, K] f32 = grad_output[M, N]^T x[M, K] (bf16, 2-D, unit column stride)."""
     dev = _require_cuda("weight_grad", grad_output, x)

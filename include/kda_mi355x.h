@@ -539,6 +539,69 @@ int kda_embedding_backward(int64_t n_tokens, int32_t vocab, int32_t dim, const i
                            const void* grad_output, void* grad_weight, hipStream_t stream);
 
 /*
+ * Post-training: losses on the log-probabilities of given tokens under soft-capped logits, the
+ * bf16 logits [rows, stride], vocab and softcap of kda_softcap_cross_entropy_forward.  Rows whose
+ * target is ignore_index are not read; their outputs and gradient rows are zero.  A target outside
+ * [0, vocab) or a NaN logit makes that row's outputs NaN.  No counterparts in the reference (its
+ * trainer has the cross entropy alone).
+ *
+ * log_probs[r] = z[r, t_r] - lse_r (f32, and / or f64 in log_probs64: either may be NULL), lse_rows
+ * as the cross entropy's (NULL: not written), entropy_rows[r] = lse_r - sum_j p_j z_j (NULL: not
+ * computed).
+ */
+int kda_softcap_log_probs_forward(int64_t rows, int32_t vocab, int64_t stride, float softcap,
+                                  const void* logits, const int64_t* targets, int64_t ignore_index,
+                                  float* log_probs, double* log_probs64, float* lse_rows,
+                                  float* entropy_rows, hipStream_t stream);
+
+/*
+ * Backward of the above: grad_logits [rows, stride] bf16 = (1 - (z / softcap)^2) *
+ *   (g_r ([j = t_r] - p_j) - h_r p_j (z_j - lse_r + entropy_r)), zero in padding columns,
+ * for row gradients g_rows of the log-probabilities and h_rows of the entropies (f32; either may
+ * be NULL), both times the device scalar scale (NULL: 1).  Rows with zero gradients are not read.
+ */
+int kda_softcap_log_probs_backward(int64_t rows, int32_t vocab, int64_t stride, float softcap,
+                                   const void* logits, const int64_t* targets, int64_t ignore_index,
+                                   const float* lse_rows, const float* entropy_rows, const float* g_rows,
+                                   const float* h_rows, const float* scale, void* grad_logits,
+                                   hipStream_t stream);
+
+/*
+ * Clipped policy loss of given log-probabilities (f32 [rows], as all row inputs):
+ *   loss = sum_r w_r (-min(q_r A_r, clip(q_r, clip_lo, clip_hi) A_r) + kl_coef k_r),
+ *   q = exp(log_probs - old_log_probs),  d = ref_log_probs - log_probs,  k = e^d - d - 1
+ * (ref_log_probs NULL: k = 0), w_r = weights[r], or 1 / number of rows with a target (NULL).
+ * stats [2] = sum_r w_r k_r and the weight of the rows where clipping is in force; slope_rows
+ * (NULL: not written) = d loss / d log_probs.  Rows without a target or of weight 0 count
+ * nothing.  Fixed-order f64 sums in one workgroup.
+ */
+int kda_policy_rows(int64_t rows, const int64_t* targets, int64_t ignore_index, const float* log_probs,
+                    const float* old_log_probs, const float* advantages, const float* ref_log_probs,
+                    const float* weights, float clip_lo, float clip_hi, float kl_coef, float* loss,
+                    float* stats, float* slope_rows, hipStream_t stream);
+
+/* Bytes of scratch kda_preference_pairs needs. */
+size_t kda_preference_pairs_scratch_bytes(int32_t pairs);
+
+/*
+ * Preference loss of pairs of sequences given their rows' log-probabilities (f64 [rows], 0 without
+ * a target).  Sequence s of 2 * pairs holds rows s * seq_len .., or cu_seqlens[s] ..
+ * cu_seqlens[s + 1] - 1 (device int32, NULL: equal lengths); sequence i < pairs is the chosen one
+ * of pair i, pairs + i the rejected one.
+ *   seq_log_probs[s] = sum of its rows (average: their mean over rows with a target)
+ *   margins[i] = beta * ((seq_i - ref_i) - (seq_{pairs+i} - ref_{pairs+i}))   (ref_log_probs NULL: 0)
+ *   loss = mean_i -(1 - label_smoothing) log sigmoid(m_i) - label_smoothing log sigmoid(-m_i)
+ * slope_rows (NULL: not written) = d loss / d log-probability of the row, 0 outside every sequence.
+ * cu_seqlens that are negative, decreasing or beyond rows make every output NaN.  Fixed-order f64
+ * sums in one workgroup.
+ */
+int kda_preference_pairs(int64_t rows, int64_t seq_len, int32_t pairs, const int32_t* cu_seqlens,
+                         const int64_t* targets, int64_t ignore_index, const double* log_probs64,
+                         const float* ref_log_probs, float beta, float label_smoothing, int32_t average,
+                         float* loss, float* seq_log_probs, float* margins, float* slope_rows,
+                         void* scratch, hipStream_t stream);
+
+/*
  * Measurement only (no counterpart in the reference): launches `workgroups` workgroups of
  * four waves; each wave runs `iters` rounds of 8 x 16,384 FLOP of bf16 MFMAs in independent
  * chains with no memory traffic (shape 0: v_mfma_f32_16x16x32_bf16, 8 chains; shape 1:
