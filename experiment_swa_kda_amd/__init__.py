@@ -7,14 +7,16 @@ from .kda import (  # noqa: F401
     KDAState,
     KimiDeltaAttention,
     Linear,
+    LoraLinear,
     RMSNormGated,
     ShortConvolution,
     k3_decay_gate,
     kda,
     kda_backend_provenance,
+    lora_linear,
     prepare_kda_backend,
     project_runtime_events,
     reset_project_runtime_events,
 )
 
-__all__ = ["KDAState", "KimiDeltaAttention", "k3_decay_gate", "kda", "prepare_kda_backend"]
+__all__ = ["KDAState", "KimiDeltaAttention", "LoraLinear", "k3_decay_gate", "kda", "lora_linear", "prepare_kda_backend"]

@@ -32,6 +32,7 @@ from dataclasses import dataclass
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 from torch.nn.modules import module as _module
 from torch.overrides import _get_current_function_mode_stack
 from torch.utils._device import DeviceContext
@@ -211,6 +212,113 @@ def linear_few_rows(m, x, *, relu2=False, residual=None):
     if residual is not None and residual.dtype != x.dtype:
         return None
     return ops.linear_rows(x, w16, relu2=relu2, residual=residual)
+
+
+class _LoraLinear(torch.autograd.Function):
+    """y = x W^T + s_a (x A_a^T) B_a^T, a the adapter of the row: the adapters' part is formed first
+    and the shared projection added to it, so y is rounded once more than a plain projection.
+    bf16 W, A and B (casts of the masters, whose gradients come back in f32)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, a, b, ids, scaling, w16, a16, b16):
+        x2 = x.reshape(-1, x.shape[-1])
+        u = ops.lora_shrink(x2, a16, ids, scaling)
+        y = ops.lora_expand(u, b16, ids, factor_cols=True).addmm_(x2, w16.t())
+        ctx.save_for_backward(x2, w16, a16, b16, ids, scaling, u)
+        ctx.shape, ctx.types = x.shape, (weight.dtype, a.dtype, b.dtype)
+        return y.view(*x.shape[:-1], w16.shape[0])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x2, w16, a16, b16, ids, scaling, u = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        g2 = grad.reshape(-1, grad.shape[-1]).to(torch.bfloat16)
+        dx = dw = da = db = None
+        if need[0] or need[2]:
+            t = ops.lora_shrink(g2, b16, ids, scaling, factor_cols=True)
+            if need[0]:
+                dx = ops.lora_expand(t, a16, ids).addmm_(g2, w16).view(ctx.shape)
+            if need[2]:
+                da = ops.lora_grad(x2, t, ids, a16.shape[0]).to(ctx.types[1])
+        if need[1]:
+            dw = (ops.weight_grad(g2, x2) if w16.numel() <= _SPLIT_WGRAD_MAX else _mm_f32(g2.t(), x2)).to(ctx.types[0])
+        if need[3]:
+            db = ops.lora_grad(g2, u, ids, b16.shape[0], out_cols=True).to(ctx.types[2])
+        return dx, dw, da, db, None, None, None, None, None
+
+
+def _check_lora(x, weight, a, b, ids, scaling):
+    """The checks of lora_linear; returns ids as int32."""
+    K = x.shape[-1] if x.ndim else 0
+    if x.ndim < 2 or weight.ndim != 2 or weight.shape[1] != K:
+        raise ValueError("lora_linear: x [..., K] and weight [N, K] expected")
+    if a.ndim != 3 or b.ndim != 3 or a.shape[0] != b.shape[0] or a.shape[2] != K or b.shape != (a.shape[0], weight.shape[0], a.shape[1]):
+        raise ValueError("lora_linear: lora_a [n, R, K] and lora_b [n, N, R] expected")
+    if scaling.shape != a.shape[:1]:
+        raise ValueError(f"lora_linear: scaling must have shape {tuple(a.shape[:1])}")
+    if ids.dtype not in (torch.int32, torch.int64) or ids.shape not in (x.shape[:1], x.shape[:-1]):
+        raise ValueError("lora_linear: adapter_ids int32, one for each sequence (x.shape[:1]) or row (x.shape[:-1])")
+    return ids if ids.dtype == torch.int32 else ids.clamp(-1, a.shape[0]).to(torch.int32)
+
+
+def lora_linear(x, weight, lora_a, lora_b, adapter_ids, scaling):
+    """``x @ weight.T`` plus every row's own low-rank adapter: ``scaling[a] (x @ lora_a[a].T) @
+    lora_b[a].T`` with a = ``adapter_ids`` of the row's sequence (ids shaped ``x.shape[:1]``) or of
+    the row itself (``x.shape[:-1]``); an id outside [0, n), such as -1, means no adapter.
+
+    x [..., K]; weight [N, K]; lora_a [n, R, K], lora_b [n, N, R] and scaling [n] hold the n adapters.
+    bf16 x on the GPU runs the HIP kernels (K, N and R multiples of 8, R at most 128, or RuntimeError)
+    with weight and adapters rounded to bf16 where they are f32 masters, as ``Linear``'s; anything
+    else runs the eager form in x's type.  Gradients reach x, weight, lora_a and lora_b, in their own
+    types; scaling is a constant."""
+    ids = _check_lora(x, weight, lora_a, lora_b, adapter_ids, scaling)
+    if x.is_cuda and x.dtype == torch.bfloat16:
+        w16, a16, b16 = (t.detach().to(torch.bfloat16) for t in (weight, lora_a, lora_b))
+        return _LoraLinear.apply(x, weight, lora_a, lora_b, ids.contiguous(), scaling.detach().float(), w16, a16, b16)
+    return _lora_eager(x, weight, lora_a, lora_b, ids, scaling)
+
+
+def _lora_eager(x, weight, a, b, ids, scaling):
+    if ids.ndim < x.ndim - 1:
+        ids = ids.view(-1, *([1] * (x.ndim - 2))).expand(x.shape[:-1])
+    y = F.linear(x, weight.to(x.dtype))
+    for i in range(a.shape[0]):
+        here = (ids == i)[..., None]
+        xi = torch.where(here, x, 0.0)  # (another row's NaN stays out of this adapter's gradients)
+        y = y + torch.where(here, F.linear(F.linear(xi, a[i].to(x.dtype)), b[i].to(x.dtype)) * scaling[i].to(x.dtype), 0.0)
+    return y
+
+
+class LoraLinear(Linear):
+    """A ``Linear`` with a bank of n low-rank adapters, of which every sequence of a call uses its
+    own: ``adapter_ids`` (set by the caller, ``GPT.use_adapters``) is int32 with an entry for each
+    sequence or row of the input, -1 for none; None runs the shared projection alone.
+
+    Parameters ``lora_a`` [n, R, in], ``lora_b`` [n, out, R] (f32 masters, cast to bf16 per call) and
+    the buffer ``scaling`` [n].  ``lora_b`` starts at zero: a fresh adapter changes nothing."""
+
+    def __init__(self, in_features: int, out_features: int, adapters: int, rank: int, alpha: float | None = None):
+        super().__init__(in_features, out_features, bias=False)
+        self.lora_a = nn.Parameter(torch.empty(adapters, rank, in_features))
+        self.lora_b = nn.Parameter(torch.zeros(adapters, out_features, rank))
+        nn.init.uniform_(self.lora_a, -in_features ** -0.5, in_features ** -0.5)
+        self.register_buffer("scaling", torch.full((adapters,), (rank if alpha is None else alpha) / rank))
+        self.adapter_ids = None
+
+    def forward(self, x: torch.Tensor, w16: torch.Tensor | None = None) -> torch.Tensor:
+        if self.adapter_ids is None:
+            return super().forward(x, w16)
+        if not (x.is_cuda and x.dtype == torch.bfloat16):
+            return lora_linear(x, self.weight, self.lora_a, self.lora_b, self.adapter_ids, self.scaling)
+        ids = _check_lora(x, self.weight, self.lora_a, self.lora_b, self.adapter_ids, self.scaling)
+        w16 = getattr(self, "_w16", None) if w16 is None else w16
+        a16, b16 = getattr(self, "_lora16", None) or self.adapters_bf16()
+        return _LoraLinear.apply(x, self.weight, self.lora_a, self.lora_b, ids.contiguous(), self.scaling.float(),
+                                 self.weight.detach().to(torch.bfloat16) if w16 is None else w16, a16, b16)
+
+    def adapters_bf16(self):
+        return tuple(t.detach().to(torch.bfloat16) for t in (self.lora_a, self.lora_b))
 
 
 def _norm_gate_eager(x, gate, weight, eps):
@@ -1037,5 +1145,5 @@ class KimiDeltaAttention(nn.Module):
 
 
 __all__ = ["KDAState", "KimiDeltaAttention", "k3_decay_gate", "kda", "kda_norm_gate", "prepare_kda_backend",
-           "ShortConvolution", "RMSNormGated", "Linear", "kda_backend_provenance",
+           "ShortConvolution", "RMSNormGated", "Linear", "LoraLinear", "lora_linear", "kda_backend_provenance",
            "project_runtime_events", "reset_project_runtime_events"]

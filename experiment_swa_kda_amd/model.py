@@ -25,7 +25,7 @@ import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
 from . import ops
-from .kda import KDAState, KimiDeltaAttention, Linear, linear_few_rows, plain
+from .kda import KDAState, KimiDeltaAttention, Linear, LoraLinear, linear_few_rows, plain
 
 
 @dataclass
@@ -697,6 +697,9 @@ class GPT(nn.Module):
                 if isinstance(m, Linear) and m.weight.dtype == torch.float32 and id(m.weight) not in stacked:
                     m._w16 = m.weight.to(torch.bfloat16)
                     out.append(m._w16)
+                if isinstance(m, LoraLinear):
+                    m._lora16 = m.adapters_bf16()
+                    out += m._lora16
         return out
 
     def drop_bf16_weights(self) -> None:
@@ -707,6 +710,33 @@ class GPT(nn.Module):
                 m._w16_of = None
             if isinstance(m, Linear):
                 m._w16 = None
+            if isinstance(m, LoraLinear):
+                m._lora16 = None
+
+    def add_adapters(self, adapters: int, rank: int, alpha: float | None = None) -> list:
+        """Gives the projections behind the mixers (``o_proj``), those of the MLPs and the head a bank of
+        low-rank adapters beside their weights (``LoraLinear``; the mixers' input projections run stacked
+        and keep theirs alone).  Returns the new parameters: train these, the rest frozen, with
+        ``use_adapters`` naming the adapter of every sequence."""
+        new = []
+        for owner, name in [(b.attn, "o_proj") for b in self.transformer.h] + [
+                (b.mlp, name) for b in self.transformer.h for name in ("c_fc", "c_proj")] + [(self, "lm_head")]:
+            old = getattr(owner, name)
+            if type(old) is not Linear:
+                raise ValueError(f"add_adapters: {name} is no plain Linear (adapters are added once)")
+            m = LoraLinear(old.in_features, old.out_features, adapters, rank, alpha).to(old.weight.device)
+            m.weight = old.weight
+            setattr(owner, name, m)
+            new += [m.lora_a, m.lora_b]
+        return new
+
+    def use_adapters(self, adapter_ids) -> None:
+        """The adapter of every sequence of the calls that follow: int32 [B] on the model's device, -1 for
+        none; None runs the shared weights alone.  The tensor is read by each call, so a captured call
+        follows what is copied into it."""
+        for m in self.modules():
+            if isinstance(m, LoraLinear):
+                m.adapter_ids = adapter_ids
 
     @torch.no_grad()
     def init_weights(self, generator=None):

@@ -808,6 +808,78 @@ def embedding_backward(idx, grad_output, vocab):
     return dw
 
 
+def _lora_rows(what, ids, rows):
+    """Rows for each entry of ids: 1 (an id a row) or as many as a sequence has."""
+    if ids.dtype != torch.int32 or not ids.is_contiguous() or (rows and (ids.numel() == 0 or rows % ids.numel())):
+        raise RuntimeError(f"{what}: contiguous int32 ids expected, each for the same number of rows")
+    return rows // ids.numel() if rows else 1
+
+
+def lora_shrink(x, factor, ids, scale, *, factor_cols=False):
+    """u [M, R] f32 = scale[a] F_a x of the rows x [M, J] bf16, a = the row's adapter (ids: one a row,
+    or one for every M / numel rows; outside [0, n): zeros).  factor [n, R, J] bf16, with
+    ``factor_cols`` [n, J, R]; scale [n] f32 or None."""
+    what = "lora_shrink"
+    dev = _require_cuda(what, x, factor, ids, scale)
+    _check_dtype(what, x, torch.bfloat16, "x")
+    _check_dtype(what, factor, torch.bfloat16, "factor")
+    _check_dtype(what, scale, torch.float32, "scale")
+    if x.ndim != 2 or factor.ndim != 3 or factor.shape[1 if factor_cols else 2] != x.shape[1]:
+        raise RuntimeError(f"{what}: x [M, J] and factor [n, R, J] (factor_cols: [n, J, R]) expected")
+    n, R, J = factor.shape[0], factor.shape[2 if factor_cols else 1], x.shape[1]
+    if scale is not None and scale.shape != (n,):
+        raise RuntimeError(f"{what}: scale must have shape {(n,)}")
+    per = _lora_rows(what, ids, x.shape[0])
+    x, factor, scale = _c(x), _c(factor), _c(scale)
+    u = torch.empty(x.shape[0], R, dtype=torch.float32, device=dev)
+    with _on(dev):
+        rc = _lib.load().kda_lora_shrink(x.shape[0], J, R, n, ptr(ids), per, ptr(x), J, ptr(factor),
+                                         1 if factor_cols else 0, ptr(scale), ptr(u), _stream(dev))
+    check(rc, "kda_lora_shrink")
+    return u
+
+
+def lora_expand(u, factor, ids, *, factor_cols=False):
+    """y [M, J] bf16 = F_a^T u of the rows u [M, R] f32; factor and ids as in :func:`lora_shrink`."""
+    what = "lora_expand"
+    dev = _require_cuda(what, u, factor, ids)
+    _check_dtype(what, u, torch.float32, "u")
+    _check_dtype(what, factor, torch.bfloat16, "factor")
+    if u.ndim != 2 or factor.ndim != 3 or factor.shape[2 if factor_cols else 1] != u.shape[1]:
+        raise RuntimeError(f"{what}: u [M, R] and factor [n, R, J] (factor_cols: [n, J, R]) expected")
+    n, J, R = factor.shape[0], factor.shape[1 if factor_cols else 2], u.shape[1]
+    per = _lora_rows(what, ids, u.shape[0])
+    u, factor = _c(u), _c(factor)
+    y = torch.empty(u.shape[0], J, dtype=torch.bfloat16, device=dev)
+    with _on(dev):
+        rc = _lib.load().kda_lora_expand(u.shape[0], J, R, n, ptr(ids), per, ptr(u), ptr(factor),
+                                         1 if factor_cols else 0, ptr(y), J, _stream(dev))
+    check(rc, "kda_lora_expand")
+    return y
+
+
+def lora_grad(x, u, ids, n, *, out_cols=False):
+    """G [n, R, J] f32 (``out_cols``: [n, J, R]), G_a = sum over adapter a's rows of u [M, R] f32 times
+    x [M, J] bf16; ids as in :func:`lora_shrink`.  Fixed-order sums."""
+    what = "lora_grad"
+    dev = _require_cuda(what, x, u, ids)
+    _check_dtype(what, x, torch.bfloat16, "x")
+    _check_dtype(what, u, torch.float32, "u")
+    if x.ndim != 2 or u.ndim != 2 or x.shape[0] != u.shape[0]:
+        raise RuntimeError(f"{what}: x [M, J] and u [M, R] expected")
+    (M, J), R = x.shape, u.shape[1]
+    per = _lora_rows(what, ids, M)
+    x, u = _c(x), _c(u)
+    lib = _lib.load()
+    scratch = torch.empty(lib.kda_lora_grad_scratch_bytes(M, J, R, n), dtype=torch.uint8, device=dev)
+    grad = torch.empty((n, J, R) if out_cols else (n, R, J), dtype=torch.float32, device=dev)
+    with _on(dev):
+        rc = lib.kda_lora_grad(M, J, R, n, ptr(ids), per, ptr(x), J, ptr(u), 1 if out_cols else 0, ptr(grad),
+                               ptr(scratch), _stream(dev))
+    check(rc, "kda_lora_grad")
+    return grad
+
+
 def softcap_cross_entropy_backward(logits, targets, lse, grad_scale, vocab, softcap, ignore_index=-1):
     """grad_scale: f32 device scalar (dL/dmean / non-ignored count) -> grad [rows, stride] bf16."""
     dev = _require_cuda("softcap_cross_entropy_backward", logits, targets, lse, grad_scale)

@@ -602,6 +602,30 @@ int kda_preference_pairs(int64_t rows, int64_t seq_len, int32_t pairs, const int
                          void* scratch, hipStream_t stream);
 
 /*
+ * Low-rank adapters of many requests beside a shared projection (no counterpart in the reference):
+ * row m of x belongs to adapter a(m) = ids[m / rows_per_id] (device int32; none where that lies
+ * outside [0, n)).  The three products of y_m = W x_m + s B (A x_m) and its gradients with a
+ * factor F of adapter a(m), J its long dimension (a multiple of 8), R the rank (a multiple of 8, at
+ * most 128); factor [n, R, J] bf16, or [n, J, R] with factor_cols:
+ *   shrink  u[m, r] = scale[a(m)] sum_j F[r, j] x[m, j]   f32 [M, R], zero rows without an adapter
+ *                                                         (scale NULL: 1)
+ *   expand  y[m, j] = sum_r F[r, j] u[m, r]               bf16 [M, J], zero rows without an adapter
+ *   grad    G[a][r, j] = sum over rows of a of u[m, r] x[m, j]   f32 [n, R, J] ([n, J, R] with
+ *           out_cols), zero for adapters without rows; fixed-order sums
+ * x and y have row strides ldx, ldy (multiples of 8).
+ */
+int kda_lora_shrink(int64_t M, int32_t J, int32_t R, int32_t n, const int32_t* ids, int64_t rows_per_id,
+                    const void* x, int64_t ldx, const void* factor, int32_t factor_cols, const float* scale,
+                    float* u, hipStream_t stream);
+int kda_lora_expand(int64_t M, int32_t J, int32_t R, int32_t n, const int32_t* ids, int64_t rows_per_id,
+                    const float* u, const void* factor, int32_t factor_cols, void* y, int64_t ldy,
+                    hipStream_t stream);
+size_t kda_lora_grad_scratch_bytes(int64_t M, int32_t J, int32_t R, int32_t n);
+int kda_lora_grad(int64_t M, int32_t J, int32_t R, int32_t n, const int32_t* ids, int64_t rows_per_id,
+                  const void* x, int64_t ldx, const float* u, int32_t out_cols, float* grad, void* scratch,
+                  hipStream_t stream);
+
+/*
  * Measurement only (no counterpart in the reference): launches `workgroups` workgroups of
  * four waves; each wave runs `iters` rounds of 8 x 16,384 FLOP of bf16 MFMAs in independent
  * chains with no memory traffic (shape 0: v_mfma_f32_16x16x32_bf16, 8 chains; shape 1:

@@ -78,3 +78,21 @@ def preference(logp, targets, starts, ref, beta, smoothing, average, ignore=-1):
         for r in s:
             slope[r] = (dm[i] if i < pairs else -dm[i - pairs]) / n
     return loss, seq, m, slope
+
+
+def lora(x, w, a, b, ids, scale, dy=None):
+    """y = x W^T + s (x A^T) B^T of rows [M, K] with row ids, and for dy (dx, dW, dA, dB)."""
+    y = x @ w.T
+    for m, i in enumerate(ids):
+        if 0 <= i < len(a):
+            y[m] += scale[i] * (b[i] @ (a[i] @ x[m]))
+    if dy is None:
+        return y
+    dx, da, db = dy @ w, np.zeros_like(a), np.zeros_like(b)
+    for m, i in enumerate(ids):
+        if 0 <= i < len(a):
+            t = scale[i] * (dy[m] @ b[i])
+            dx[m] += t @ a[i]
+            da[i] += np.outer(t, x[m])
+            db[i] += scale[i] * np.outer(dy[m], a[i] @ x[m])
+    return y, dx, dy.T @ x, da, db
