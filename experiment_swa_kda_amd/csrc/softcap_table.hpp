@@ -34,13 +34,17 @@ typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 // arithmetic: clamp(bits & 0x7fff) - (kTabELo << 7) + sign * kTabHalf, both < 2^14.  The fast
 // paths drop the constant - (kTabELo << 7) (tab_index2_biased) and index a table pointer
 // moved back by it instead.
-__device__ __forceinline__ void tab_index2_biased(unsigned w, int& lo, int& hi) {
+__device__ __forceinline__ unsigned tab_index2_packed(unsigned w) {  // both, biased, in one word
   u16x2 k = __builtin_bit_cast(u16x2, w & 0x7fff7fffu);
   k = __builtin_elementwise_max(k, (u16x2)(kTabELo << 7));
   k = __builtin_elementwise_min(k, (u16x2)((kTabEHi << 7) | 127));
   const u16x2 sg = __builtin_bit_cast(u16x2, (w >> 15) & 0x00010001u);
   const u16x2 idx = k + sg * (u16x2)kTabHalf;  // < 17408 + 4224
-  const unsigned r = __builtin_bit_cast(unsigned, idx);
+  return __builtin_bit_cast(unsigned, idx);
+}
+
+__device__ __forceinline__ void tab_index2_biased(unsigned w, int& lo, int& hi) {
+  const unsigned r = tab_index2_packed(w);
   lo = (int)(r & 0xffffu);
   hi = (int)(r >> 16);
 }

@@ -237,6 +237,33 @@ class _PolicyLoss(torch.autograd.Function):
                 *(None,) * 12)
 
 
+class _PolicyLossFused(torch.autograd.Function):
+    """The same loss with its gradient formed in the forward pass, in one read of the logits, for an
+    assumed upstream gradient ``expected_grad``; the backward returns that buffer, rescaled on the
+    device only if the actual upstream gradient differs."""
+
+    @staticmethod
+    def forward(ctx, logits, targets, old, adv, ref, weights, vocab, softcap, ignore_index, lo, hi, kl_coef,
+                expected_grad):
+        loss, stats, logp, dlogits = ops.policy_fused(logits, targets, old, adv, ref, weights, vocab, softcap, lo, hi,
+                                                      kl_coef, ignore_index, expected_grad=expected_grad)
+        ctx.save_for_backward(dlogits)
+        ctx.expected = expected_grad
+        ctx.used = False
+        ctx.mark_non_differentiable(logp, stats)
+        return loss, logp, stats
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad, _logp, _stats):
+        if ctx.used:  # the gradient buffer is handed out (and rescaled) in place
+            raise RuntimeError("policy_loss: the fused form's backward can run only once")
+        ctx.used = True
+        (dlogits,) = ctx.saved_tensors
+        ops.rescale_bf16_if_changed(dlogits, grad, ctx.expected)
+        return (dlogits, *(None,) * 12)
+
+
 class _PreferenceLoss(torch.autograd.Function):
     """The preference loss on the HIP kernels: the log-probability pass, one kernel over sequences
     and pairs that leaves every row's slope, and the logit gradient for those slopes."""
@@ -306,7 +333,7 @@ class PolicyLoss(NamedTuple):
 
 
 def policy_loss(logits, targets, old_log_probs, advantages, vocab, softcap=15.0, ignore_index=-1, *,
-                ref_log_probs=None, clip=0.2, clip_high=None, kl_coef=0.0, weights=None):
+                ref_log_probs=None, clip=0.2, clip_high=None, kl_coef=0.0, weights=None, expected_grad=1.0):
     """Clipped policy loss over the tokens ``targets`` of sampled sequences, with soft-capped
     logits [..., columns]:
 
@@ -317,7 +344,10 @@ def policy_loss(logits, targets, old_log_probs, advantages, vocab, softcap=15.0,
     there is none, as the cross entropy's).  Rows without a target or of weight 0 are not counted (their
     log_probs are 0).
     clip_high defaults to clip.  The row tensors are shaped like targets and are constants.
-    Returns a PolicyLoss."""
+    bf16 CUDA logits run the HIP kernels, anything else the eager f32 form.  With a gradient to form
+    and rows of at most 32768 columns it is formed in the forward pass for ``expected_grad``, the
+    dL/dloss the caller will back-propagate (another one costs a pass over it; the backward can run
+    once); None forms it in the backward.  Returns a PolicyLoss."""
     flat, t, old, adv, ref, w = _flat_tokens("policy_loss", logits, targets, vocab, old_log_probs, advantages,
                                              ref_log_probs, weights)
     clip_high = clip if clip_high is None else clip_high
@@ -327,8 +357,12 @@ def policy_loss(logits, targets, old_log_probs, advantages, vocab, softcap=15.0,
     if logits.is_cuda and logits.dtype == torch.bfloat16:
         if w is not None:  # rows of weight 0 need not be read
             t = torch.where(w != 0, t, ignore_index)
-        loss, logp, stats = _PolicyLoss.apply(flat, t, old, adv, ref, w, vocab, float(softcap), ignore_index, lo, hi,
-                                              float(kl_coef), torch.is_grad_enabled() and logits.requires_grad)
+        grad = torch.is_grad_enabled() and logits.requires_grad
+        args = (flat, t, old, adv, ref, w, vocab, float(softcap), ignore_index, lo, hi, float(kl_coef))
+        if grad and expected_grad and flat.shape[0] and ops.policy_fused_supported(flat.shape[1]):
+            loss, logp, stats = _PolicyLossFused.apply(*args, float(expected_grad))
+        else:
+            loss, logp, stats = _PolicyLoss.apply(*args, grad)
         return PolicyLoss(loss, logp.view(targets.shape), stats[0], stats[1])
     if w is not None:
         t = torch.where(w != 0, t, ignore_index)

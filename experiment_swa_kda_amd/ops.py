@@ -977,6 +977,38 @@ def policy_rows(targets, log_probs, old_log_probs, advantages, ref_log_probs, we
     return loss, stats, slope
 
 
+def policy_fused_supported(stride):
+    """True where the one-pass policy loss takes rows of this many columns (at most 32768)."""
+    return bool(_lib.load().kda_policy_fused_supported(int(stride)))
+
+
+def policy_fused(logits, targets, old_log_probs, advantages, ref_log_probs, weights, vocab, softcap, clip_lo, clip_hi,
+                 kl_coef, ignore_index=-1, *, expected_grad=1.0):
+    """Policy loss and logit gradient in one read of the logits [rows, stride] bf16, rows > 0 ->
+    (loss, stats [2], log-probabilities [rows], grad_logits for an upstream gradient of
+    ``expected_grad``: rescale it with rescale_bf16_if_changed when the actual one differs)."""
+    what = "policy_fused"
+    if old_log_probs is None or advantages is None:
+        raise RuntimeError(f"{what}: old_log_probs and advantages [rows] expected")
+    dev = _token_inputs(what, logits, targets, old_log_probs, advantages, ref_log_probs, weights)
+    logits, targets, old_log_probs, advantages, ref_log_probs, weights = (
+        _c(t) for t in (logits, targets, old_log_probs, advantages, ref_log_probs, weights))
+    rows, stride = logits.shape
+    lib = _lib.load()
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    stats = torch.empty(2, dtype=torch.float32, device=dev)
+    logp = torch.empty(rows, dtype=torch.float32, device=dev)
+    grad = torch.empty_like(logits)
+    with _on(dev):
+        scratch = torch.empty(lib.kda_policy_fused_scratch_bytes(rows, stride), dtype=torch.uint8, device=dev)
+        rc = lib.kda_policy_fused(
+            rows, int(vocab), stride, float(softcap), ptr(logits), ptr(targets), int(ignore_index), ptr(old_log_probs),
+            ptr(advantages), ptr(ref_log_probs), ptr(weights), float(clip_lo), float(clip_hi), float(kl_coef),
+            float(expected_grad), ptr(loss), ptr(stats), ptr(logp), ptr(grad), ptr(scratch), _stream(dev))
+    check(rc, "kda_policy_fused")
+    return loss, stats, logp, grad
+
+
 def preference_pairs(targets, log_probs64, pairs, seq_len, cu_seqlens, ref_log_probs, beta, label_smoothing, average,
                      ignore_index=-1, *, slopes=False):
     """Preference loss of f64 row log-probabilities [rows] -> (loss, sequence log-probabilities

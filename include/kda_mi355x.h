@@ -580,6 +580,20 @@ int kda_policy_rows(int64_t rows, const int64_t* targets, int64_t ignore_index, 
                     const float* weights, float clip_lo, float clip_hi, float kl_coef, float* loss,
                     float* stats, float* slope_rows, hipStream_t stream);
 
+/*
+ * Log-probabilities, policy loss and logit gradient in one read of the logits, for rows of at
+ * most 32768 columns (kda_policy_fused_supported): kda_softcap_log_probs_forward, kda_policy_rows
+ * and kda_softcap_log_probs_backward for an upstream gradient of expected_grad
+ * (kda_bf16_rescale_if_changed then makes it the actual one).  rows > 0.
+ */
+int kda_policy_fused_supported(int64_t stride);
+size_t kda_policy_fused_scratch_bytes(int64_t rows, int64_t stride);
+int kda_policy_fused(int64_t rows, int32_t vocab, int64_t stride, float softcap, const void* logits,
+                     const int64_t* targets, int64_t ignore_index, const float* old_log_probs,
+                     const float* advantages, const float* ref_log_probs, const float* weights,
+                     float clip_lo, float clip_hi, float kl_coef, float expected_grad, float* loss,
+                     float* stats, float* log_probs, void* grad_logits, void* scratch, hipStream_t stream);
+
 /* Bytes of scratch kda_preference_pairs needs. */
 size_t kda_preference_pairs_scratch_bytes(int32_t pairs);
 

@@ -183,7 +183,15 @@ def test_policy_loss_matches_oracle(rows, vocab, cols, weighted, with_ref):
     room = off * np.sum(total * (np.abs(unit) + np.abs(n(adv)) * 2 + 1)) + 1e-7
     assert abs(r.loss.item() - loss) <= room and abs(r.kl.item() - kl) <= room
     assert abs(r.clip_fraction.item() - share) <= 1e-6 * max(1.0, total.sum())
+    # the gradient is formed for an upstream gradient of 1, rounded to bf16, v (1 + a) with |a| <= 2^-8, and
+    # then times 2.5 rounded again, 2.5 v (1 + a) (1 + b): off by up to 2 2^-8 + 2^-16, two half-steps; formed
+    # for 2.5 at once, or in the backward, by one
     (grad,) = torch.autograd.grad(2.5 * r.loss, leaf)
+    grads = [(grad, 2)]
+    for expected in (2.5, None):
+        again = policy_loss(leaf, t.cuda(), cuda[0], cuda[1], vocab, CAP, expected_grad=expected, **opts)
+        assert abs(again.loss.item() - r.loss.item()) <= 1e-6 * max(1.0, abs(loss))
+        grads.append((torch.autograd.grad(2.5 * again.loss, leaf)[0], 1))
     # the slope's own error: that of the ratio and of e^d - 1, relative to |rho A| + c e^d
     ratio = np.exp(logp - n(old))
     size = total * (np.abs(ratio * n(adv)) + (0 if ref is None else 0.1 * np.exp(n(ref) - logp)))
@@ -191,9 +199,11 @@ def test_policy_loss_matches_oracle(rows, vocab, cols, weighted, with_ref):
     _, _, z, p = P.rows(n(x), t.tolist(), vocab, CAP)
     one = np.zeros_like(p)
     one[np.flatnonzero(t >= 0), t[t >= 0].numpy()] = 1
-    room = 2.0 ** -8 * 1.01 * np.abs(want[:, :vocab]) + 2.5 * 2 * (size[:, None] * off + np.abs(slope)[:, None] * off) * (p + one)
-    assert np.all(np.abs(n(grad)[:, :vocab] - want[:, :vocab]) <= room + 1e-38)
-    assert not n(grad)[:, vocab:].any() and not n(grad)[t.numpy() < 0].any()
+    for grad, roundings in grads:
+        room = roundings * 2.0 ** -8 * 1.01 * np.abs(want[:, :vocab]) + \
+            2.5 * 2 * (size[:, None] * off + np.abs(slope)[:, None] * off) * (p + one)
+        assert np.all(np.abs(n(grad)[:, :vocab] - want[:, :vocab]) <= room + 1e-38)
+        assert not n(grad)[:, vocab:].any() and not n(grad)[t.numpy() < 0].any()
     with torch.no_grad():
         plain = policy_loss(x.cuda(), t.cuda(), cuda[0], cuda[1], vocab, CAP, **opts)
     assert abs(plain.loss.item() - loss) <= 1e-4 * max(1, abs(loss))
