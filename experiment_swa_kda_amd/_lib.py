@@ -106,6 +106,8 @@ SIGNATURES = {
     "kda_policy_fused_supported": (ctypes.c_int, [_L]),
     "kda_policy_fused_scratch_bytes": (ctypes.c_size_t, [_L, _L]),
     "kda_policy_fused": (ctypes.c_int, [_L, _I, _L, _F, _P, _P, _L, _P, _P, _P, _P] + [_F] * 4 + [_P] * 6),
+    "kda_lora_linear_rows": (ctypes.c_int, [_I, _I, _I, _I, _I, _P, _L, _P, _L] + [_P] * 7),
+    "kda_lora_linear": (ctypes.c_int, [_L, _I, _I, _I, _I, _P, _L, _P, _L, _P, _I, _P, _P, _P, _P]),
     "kda_lora_shrink": (ctypes.c_int, [_L, _I, _I, _I, _P, _L, _P, _L, _P, _I, _P, _P, _P]),
     "kda_lora_expand": (ctypes.c_int, [_L, _I, _I, _I, _P, _L, _P, _P, _I, _P, _L, _P]),
     "kda_lora_grad_scratch_bytes": (ctypes.c_size_t, [_L, _I, _I, _I]),

@@ -25,12 +25,13 @@ LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 
 SOURCES = ["capi.cpp", "decode.hip", "conv.hip", "norm_gate.hip", "chunk_fwd.hip", "chunk_bwd.hip", "softcap_ce.hip",
            "weight_grad.hip", "trainer_ops.hip", "linear_rows.hip", "mfma_probe.hip", "generic.hip",
-           "token_loss.hip", "lora.hip"]
+           "token_loss.hip", "lora.hip", "lora_linear.hip"]
 # Per-source extra flags.  The chunk kernels keep MFMA accumulators in VGPRs: their
 # accumulators feed VALU work every step, and the AGPR form costs a copy per element.
 EXTRA_FLAGS = {
     "chunk_fwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "chunk_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "lora_linear.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 ARCH = "gfx950"
 

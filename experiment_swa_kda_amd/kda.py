@@ -214,16 +214,26 @@ def linear_few_rows(m, x, *, relu2=False, residual=None):
     return ops.linear_rows(x, w16, relu2=relu2, residual=residual)
 
 
+def _lora_forward(x2, w16, a16, b16, ids, scaling):
+    """(y, u) = (x W^T + u B_a^T, s_a x A_a^T) of the rows x2 [M, K], a the row's adapter.  One rounding of
+    y, or for the long contractions that the library multiplies two of the adapters' part, which is
+    then formed first and the shared projection added to it."""
+    if ops.lora_linear_rows_fits(x2, w16):
+        return ops.lora_linear_rows(x2, w16, a16, b16, ids, scaling)
+    u = ops.lora_shrink(x2, a16, ids, scaling)
+    if ops.lora_linear_gains(x2.shape[0], x2.shape[1], w16.shape[0]):
+        return ops.lora_linear(x2, w16, u, b16, ids), u
+    return ops.lora_expand(u, b16, ids, factor_cols=True).addmm_(x2, w16.t()), u
+
+
 class _LoraLinear(torch.autograd.Function):
-    """y = x W^T + s_a (x A_a^T) B_a^T, a the adapter of the row: the adapters' part is formed first
-    and the shared projection added to it, so y is rounded once more than a plain projection.
-    bf16 W, A and B (casts of the masters, whose gradients come back in f32)."""
+    """A projection with adapters, for autograd: bf16 W, A and B (casts of the masters, whose gradients
+    come back in f32)."""
 
     @staticmethod
     def forward(ctx, x, weight, a, b, ids, scaling, w16, a16, b16):
         x2 = x.reshape(-1, x.shape[-1])
-        u = ops.lora_shrink(x2, a16, ids, scaling)
-        y = ops.lora_expand(u, b16, ids, factor_cols=True).addmm_(x2, w16.t())
+        y, u = _lora_forward(x2, w16, a16, b16, ids, scaling)
         ctx.save_for_backward(x2, w16, a16, b16, ids, scaling, u)
         ctx.shape, ctx.types = x.shape, (weight.dtype, a.dtype, b.dtype)
         return y.view(*x.shape[:-1], w16.shape[0])
@@ -238,7 +248,11 @@ class _LoraLinear(torch.autograd.Function):
         if need[0] or need[2]:
             t = ops.lora_shrink(g2, b16, ids, scaling, factor_cols=True)
             if need[0]:
-                dx = ops.lora_expand(t, a16, ids).addmm_(g2, w16).view(ctx.shape)
+                if ops.lora_linear_gains(*g2.shape, w16.shape[1]):
+                    dx = ops.lora_linear(g2, w16, t, a16, ids, weight_rows=True)
+                else:
+                    dx = ops.lora_expand(t, a16, ids).addmm_(g2, w16)
+                dx = dx.view(ctx.shape)
             if need[2]:
                 da = ops.lora_grad(x2, t, ids, a16.shape[0]).to(ctx.types[1])
         if need[1]:
@@ -246,6 +260,17 @@ class _LoraLinear(torch.autograd.Function):
         if need[3]:
             db = ops.lora_grad(g2, u, ids, b16.shape[0], out_cols=True).to(ctx.types[2])
         return dx, dw, da, db, None, None, None, None, None
+
+
+def _lora_linear(x, weight, a, b, ids, scaling, w16, a16, b16):
+    """The projection with adapters on the HIP kernels; outside autograd's and the transforms' sight
+    where nothing is to be recorded."""
+    ids = ids if ids.is_contiguous() else ids.contiguous()
+    scaling = scaling if scaling.dtype == torch.float32 else scaling.detach().float()
+    if not _needs_grad(x, weight, a, b) and _untransformed(x, weight, a, b, ids, scaling):
+        y, _ = _lora_forward(x.reshape(-1, x.shape[-1]), w16, a16, b16, ids, scaling)
+        return y.view(*x.shape[:-1], w16.shape[0])
+    return _LoraLinear.apply(x, weight, a, b, ids, scaling, w16, a16, b16)
 
 
 def _check_lora(x, weight, a, b, ids, scaling):
@@ -274,8 +299,8 @@ def lora_linear(x, weight, lora_a, lora_b, adapter_ids, scaling):
     types; scaling is a constant."""
     ids = _check_lora(x, weight, lora_a, lora_b, adapter_ids, scaling)
     if x.is_cuda and x.dtype == torch.bfloat16:
-        w16, a16, b16 = (t.detach().to(torch.bfloat16) for t in (weight, lora_a, lora_b))
-        return _LoraLinear.apply(x, weight, lora_a, lora_b, ids.contiguous(), scaling.detach().float(), w16, a16, b16)
+        w16, a16, b16 = [t if t.dtype == torch.bfloat16 else t.detach().to(torch.bfloat16) for t in (weight, lora_a, lora_b)]
+        return _lora_linear(x, weight, lora_a, lora_b, ids, scaling, w16, a16, b16)
     return _lora_eager(x, weight, lora_a, lora_b, ids, scaling)
 
 
@@ -314,8 +339,8 @@ class LoraLinear(Linear):
         ids = _check_lora(x, self.weight, self.lora_a, self.lora_b, self.adapter_ids, self.scaling)
         w16 = getattr(self, "_w16", None) if w16 is None else w16
         a16, b16 = getattr(self, "_lora16", None) or self.adapters_bf16()
-        return _LoraLinear.apply(x, self.weight, self.lora_a, self.lora_b, ids.contiguous(), self.scaling.float(),
-                                 self.weight.detach().to(torch.bfloat16) if w16 is None else w16, a16, b16)
+        return _lora_linear(x, self.weight, self.lora_a, self.lora_b, ids, self.scaling,
+                            self.weight.detach().to(torch.bfloat16) if w16 is None else w16, a16, b16)
 
     def adapters_bf16(self):
         return tuple(t.detach().to(torch.bfloat16) for t in (self.lora_a, self.lora_b))

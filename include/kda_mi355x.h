@@ -621,8 +621,8 @@ int kda_preference_pairs(int64_t rows, int64_t seq_len, int32_t pairs, const int
  * outside [0, n)).  The three products of y_m = W x_m + s B (A x_m) and its gradients with a
  * factor F of adapter a(m), J its long dimension (a multiple of 8), R the rank (a multiple of 8, at
  * most 128); factor [n, R, J] bf16, or [n, J, R] with factor_cols:
- *   shrink  u[m, r] = scale[a(m)] sum_j F[r, j] x[m, j]   f32 [M, R], zero rows without an adapter
- *                                                         (scale NULL: 1)
+ *   shrink  u[m, r] = scale[a(m)] sum_j F[r, j] x[m, j]   zero rows without an adapter (scale NULL: 1);
+ *           an f32 value as the sum of three bf16 parts, u [3, M, R]
  *   expand  y[m, j] = sum_r F[r, j] u[m, r]               bf16 [M, J], zero rows without an adapter
  *   grad    G[a][r, j] = sum over rows of a of u[m, r] x[m, j]   f32 [n, R, J] ([n, J, R] with
  *           out_cols), zero for adapters without rows; fixed-order sums
@@ -630,13 +630,30 @@ int kda_preference_pairs(int64_t rows, int64_t seq_len, int32_t pairs, const int
  */
 int kda_lora_shrink(int64_t M, int32_t J, int32_t R, int32_t n, const int32_t* ids, int64_t rows_per_id,
                     const void* x, int64_t ldx, const void* factor, int32_t factor_cols, const float* scale,
-                    float* u, hipStream_t stream);
+                    void* u, hipStream_t stream);
 int kda_lora_expand(int64_t M, int32_t J, int32_t R, int32_t n, const int32_t* ids, int64_t rows_per_id,
-                    const float* u, const void* factor, int32_t factor_cols, void* y, int64_t ldy,
+                    const void* u, const void* factor, int32_t factor_cols, void* y, int64_t ldy,
                     hipStream_t stream);
+/*
+ * The whole of y = x W^T + s B (A x) for at most 64 rows (in_dim a multiple of 32): weight
+ * [out_dim, in_dim], lora_a [n, R, in_dim], lora_b [n, out_dim, R] bf16, rounded once; u [3, rows,
+ * R] receives s A x.
+ */
+int kda_lora_linear_rows(int32_t rows, int32_t out_dim, int32_t in_dim, int32_t R, int32_t n,
+                         const int32_t* ids, int64_t rows_per_id, const void* x, int64_t x_row_stride,
+                         const void* weight, const void* lora_a, const void* lora_b, const float* scale,
+                         void* u, void* y, hipStream_t stream);
+/*
+ * y [M, N] = x [M, K] W^T + u F_a (weight [N, K], factor [n, N, R]), or with weight_rows y = x W +
+ * u F_a (weight [K, N], factor [n, R, N]), u as kda_lora_shrink leaves it; one rounding.
+ * N and K multiples of 8, at most 2^20.
+ */
+int kda_lora_linear(int64_t M, int32_t N, int32_t K, int32_t R, int32_t n, const int32_t* ids,
+                    int64_t rows_per_id, const void* x, int64_t ldx, const void* weight,
+                    int32_t weight_rows, const void* u, const void* factor, void* y, hipStream_t stream);
 size_t kda_lora_grad_scratch_bytes(int64_t M, int32_t J, int32_t R, int32_t n);
 int kda_lora_grad(int64_t M, int32_t J, int32_t R, int32_t n, const int32_t* ids, int64_t rows_per_id,
-                  const void* x, int64_t ldx, const float* u, int32_t out_cols, float* grad, void* scratch,
+                  const void* x, int64_t ldx, const void* u, int32_t out_cols, float* grad, void* scratch,
                   hipStream_t stream);
 
 /*
