@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libkda_mi35
 KDA_OK = 0
 KDA_GATE_K3 = 0
 KDA_GATE_LOGDECAY = 1
+KDA_LORA_ROWS, KDA_LORA_WHOLE, KDA_LORA_PART = 0, 1, 2
 
 # exported symbol -> (restype, argtypes); mirrors include/kda_mi355x.h
 _P = ctypes.c_void_p
@@ -108,6 +109,9 @@ SIGNATURES = {
     "kda_policy_fused": (ctypes.c_int, [_L, _I, _L, _F, _P, _P, _L, _P, _P, _P, _P] + [_F] * 4 + [_P] * 6),
     "kda_lora_linear_rows": (ctypes.c_int, [_I, _I, _I, _I, _I, _P, _L, _P, _L] + [_P] * 7),
     "kda_lora_linear": (ctypes.c_int, [_L, _I, _I, _I, _I, _P, _L, _P, _L, _P, _I, _P, _P, _P, _P]),
+    "kda_lora_forward": (ctypes.c_int, [_L, _I, _I, _I, _I, _P, _L, _P, _L, _P, _P, _P, _P, _I, _P, _P, _P]),
+    "kda_lora_backward_scratch_bytes": (ctypes.c_size_t, [_L, _I, _I, _I, _I]),
+    "kda_lora_backward": (ctypes.c_int, [_L, _I, _I, _I, _I, _P, _L, _P, _L, _P, _L] + [_P] * 5 + [_I] + [_P] * 6),
     "kda_lora_shrink": (ctypes.c_int, [_L, _I, _I, _I, _P, _L, _P, _L, _P, _I, _P, _P, _P]),
     "kda_lora_expand": (ctypes.c_int, [_L, _I, _I, _I, _P, _L, _P, _P, _I, _P, _L, _P]),
     "kda_lora_grad_scratch_bytes": (ctypes.c_size_t, [_L, _I, _I, _I]),

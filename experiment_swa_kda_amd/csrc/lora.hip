@@ -313,28 +313,29 @@ __global__ __launch_bounds__(256) void lora_expand_rows_kernel(LoraRows rows, in
 }
 
 // ---------------------------------------------------------------------------------------
-// grad: workgroup (128 columns of J, adapter, range of rows) walks the 32-row steps of its range
-// that hold a row of the adapter, with the other rows masked, and leaves an f32 partial and a
-// flag; a second kernel sums the flagged partials in order.  A single range is the result itself
-// (flag null).  COLS: the result is [n, J, R], else [n, R, J].
+// grad: workgroup (128 columns of J, adapter, range of rows) walks the 64-row steps of its range
+// that hold a row of the adapter, with the other rows masked and the next step's loads in flight, and
+// leaves an f32 partial and a flag; a second kernel sums the flagged partials in order.  A single
+// range is the result itself (flag null).  COLS: the result is [n, J, R], else [n, R, J].
 // ---------------------------------------------------------------------------------------
 constexpr int kGradCols = 128;
-constexpr int kGradWindow = 64;  // 32-row steps whose ids are looked at together
+constexpr int kGradRows = 64;
+constexpr int kGradWindow = 32;  // steps whose ids are looked at together
 
 template <int RT, bool COLS>
 __global__ __launch_bounds__(256) void lora_grad_kernel(LoraRows rows, int J, int R, const bf16* __restrict__ x,
                                                         long ldx, const bf16* __restrict__ u, int range,
                                                         float* __restrict__ part, int32_t* __restrict__ flag) {
   constexpr int XP = kGradCols + 8, UP = 16 * RT + 8;  // pitches: 16-byte rows, 4 banks apart
-  constexpr int XV = 32 * kGradCols / 8 / 256;         // vectors of a step and thread
-  constexpr int UV = (3 * 32 * 2 * RT + 255) / 256;
-  __shared__ __attribute__((aligned(16))) bf16 sx[32 * XP];
-  __shared__ __attribute__((aligned(16))) bf16 su[3][32 * UP];
+  constexpr int XV = kGradRows * kGradCols / 8 / 256;  // vectors of a step and thread
+  constexpr int UN = 3 * kGradRows * 2 * RT, UV = (UN + 255) / 256;
+  __shared__ __attribute__((aligned(16))) bf16 sx[kGradRows * XP];
+  __shared__ __attribute__((aligned(16))) bf16 su[3][kGradRows * UP];
   __shared__ int s_any[kGradWindow];
-  __shared__ int s_id[32 * kGradWindow];
+  __shared__ int s_id[kGradRows * kGradWindow];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
   const int j0 = kGradCols * blockIdx.x, a = blockIdx.y, split = blockIdx.z;
-  const int mb = split * range, me = min(rows.M, mb + range), steps = (me - mb + 31) / 32;
+  const int mb = split * range, me = min(rows.M, mb + range), steps = (me - mb + kGradRows - 1) / kGradRows;
   f32x4 acc[RT][2];
 #pragma unroll
   for (int r = 0; r < RT; ++r)
@@ -344,11 +345,11 @@ __global__ __launch_bounds__(256) void lora_grad_kernel(LoraRows rows, int J, in
   for (int w0 = 0; w0 < steps; w0 += kGradWindow) {  // which of the next steps hold a row of the adapter
     const int wn = min(kGradWindow, steps - w0);
     __syncthreads();
-    for (int i = tid; i < 32 * wn; i += 256) {
-      const int m = mb + 32 * w0 + i, id = m < me ? rows.id(m) : -1;
+    for (int s = wave; s < wn; s += 4) {
+      const int i = kGradRows * s + lane, m = mb + kGradRows * w0 + i, id = m < me ? rows.id(m) : -1;
       s_id[i] = id;
-      const unsigned long long any = __ballot(id == a);  // 32 rows to a step, two steps to a wave
-      if (lane % 32 == 0) s_any[i / 32] = (unsigned)(any >> lane) != 0;
+      const bool any = __any(id == a);
+      if (lane == 0) s_any[s] = any;
     }
     __syncthreads();
     auto next = [&](int s) {
@@ -357,18 +358,18 @@ __global__ __launch_bounds__(256) void lora_grad_kernel(LoraRows rows, int J, in
     };
     bf16x8 vx[XV], vu[UV];
     auto load = [&](int s) {
-      const int m1 = mb + 32 * (w0 + s);
+      const int m1 = mb + kGradRows * (w0 + s);
 #pragma unroll
       for (int q = 0; q < XV; ++q) {
         const int c = q * 256 + tid, row = c / (kGradCols / 8), col = 8 * (c % (kGradCols / 8));
         // (rows of other adapters are zero: whatever they hold stays out of the products)
-        const bool in = j0 + col < J && s_id[32 * s + row] == a;
+        const bool in = j0 + col < J && s_id[kGradRows * s + row] == a;
         vx[q] = keep8(*(const bf16x8*)(x + (in ? (size_t)(m1 + row) * ldx + j0 + col : (size_t)0)), in);
       }
 #pragma unroll
       for (int q = 0; q < UV; ++q) {
-        const int c = q * 256 + tid, k = c / (64 * RT), row = c / (2 * RT) % 32, r = 8 * (c % (2 * RT));
-        const bool in = k < 3 && r < R && s_id[32 * s + row] == a;
+        const int c = q * 256 + tid, k = c / (UN / 3), row = c / (2 * RT) % kGradRows, r = 8 * (c % (2 * RT));
+        const bool in = c < UN && r < R && s_id[kGradRows * s + row] == a;
         vu[q] = keep8(*(const bf16x8*)(u + (in ? ((size_t)k * rows.M + m1 + row) * R + r : (size_t)0)), in);
       }
     };
@@ -385,23 +386,26 @@ __global__ __launch_bounds__(256) void lora_grad_kernel(LoraRows rows, int J, in
 #pragma unroll
       for (int q = 0; q < UV; ++q) {
         const int c = q * 256 + tid;
-        if (c < 3 * 64 * RT) *(bf16x8*)(su[c / (64 * RT)] + c / (2 * RT) % 32 * UP + 8 * (c % (2 * RT))) = vu[q];
+        if (c < UN) *(bf16x8*)(su[c / (UN / 3)] + c / (2 * RT) % kGradRows * UP + 8 * (c % (2 * RT))) = vu[q];
       }
       s = next(s + 1);
       if (s < wn) load(s);  // in flight over this step's products
       wait_lgkm0();
       ring_barrier();
-      bf16x8 fx[2];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) fx[t] = lds_col_frag(sx, XP, 0, 32 * wave + 16 * t, lane);
+      for (int h = 0; h < kGradRows / 32; ++h) {
+        bf16x8 fx[2];
 #pragma unroll
-      for (int r = 0; r < RT; ++r)
+        for (int t = 0; t < 2; ++t) fx[t] = lds_col_frag(sx, XP, 32 * h, 32 * wave + 16 * t, lane);
 #pragma unroll
-        for (int k = 0; k < 3; ++k) {
-          const bf16x8 fu = lds_col_frag(su[k], UP, 0, 16 * r, lane);
+        for (int r = 0; r < RT; ++r)
 #pragma unroll
-          for (int t = 0; t < 2; ++t) acc[r][t] = COLS ? mfma16(fx[t], fu, acc[r][t]) : mfma16(fu, fx[t], acc[r][t]);
-        }
+          for (int k = 0; k < 3; ++k) {
+            const bf16x8 fu = lds_col_frag(su[k], UP, 32 * h, 16 * r, lane);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) acc[r][t] = COLS ? mfma16(fx[t], fu, acc[r][t]) : mfma16(fu, fx[t], acc[r][t]);
+          }
+      }
     }
   }
   if (flag) {
@@ -421,26 +425,44 @@ __global__ __launch_bounds__(256) void lora_grad_kernel(LoraRows rows, int J, in
       }
 }
 
-// The partials of every element, in order: four lanes groups of a workgroup take every fourth one,
-// eight loads in flight, and their sums meet in LDS.
+// The flagged partials of every element, in order: a workgroup lists them, its four waves take every
+// fourth one, eight loads in flight, and their sums meet in LDS.
+constexpr int kGradList = 1024;
 __global__ __launch_bounds__(256) void lora_grad_reduce_kernel(int splits, int n, long per,
                                                                const float* __restrict__ part,
                                                                const int32_t* __restrict__ flag,
                                                                float* __restrict__ out) {
+  __shared__ int list[kGradList], s_count;
   __shared__ f32x4 red[4][kWave];
   const int a = blockIdx.y, g = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  const long i = ((long)blockIdx.x * kWave + lane) * 4, ic = i < per ? i : 0;  // per is a multiple of 64
+  const long i = ((long)blockIdx.x * kWave + lane) * 4, ic = i < per ? i : 0;
   f32x4 v = zero4();
-  for (int s0 = g; s0 < splits; s0 += 32) {
-    f32x4 p[8];
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const int s = s0 + 4 * q;
-      const bool on = s < splits && flag[s * n + a];
-      p[q] = on ? *(const f32x4*)(part + ((size_t)s * n + a) * per + ic) : zero4();
+  for (int b = 0; b < splits; b += kGradList) {
+    __syncthreads();
+    if (g == 0) {
+      int count = 0;
+      for (int s0 = b; s0 < min(splits, b + kGradList); s0 += kWave) {
+        const int s = s0 + lane;
+        const bool on = s < splits && flag[s * n + a];
+        const unsigned long long m = __ballot(on);
+        if (on) list[count + __popcll(m & ((1ull << lane) - 1))] = s;
+        count += __popcll(m);
+      }
+      if (lane == 0) s_count = count;
     }
+    __syncthreads();
+    const int count = s_count;
+    for (int k0 = g; k0 < count; k0 += 32) {
+      f32x4 p[8];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) v += p[q];
+      for (int q = 0; q < 8; ++q) {
+        const int k = k0 + 4 * q;
+        p[q] = *(const f32x4*)(part + ((size_t)list[k < count ? k : g] * n + a) * per + ic);
+        if (k >= count) p[q] = zero4();
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v += p[q];
+    }
   }
   red[g][lane] = v;
   __syncthreads();
@@ -459,7 +481,7 @@ static GradPlan grad_plan(int64_t M, int32_t J, int32_t R, int32_t n) {
   const int64_t most = ((int64_t)512 << 20) / ((int64_t)n * R * J * 4);
   if (splits > most) splits = most;
   if (splits < 1) splits = 1;
-  const int64_t range = ((M + splits - 1) / splits + 31) / 32 * 32;
+  const int64_t range = ((M + splits - 1) / splits + kGradRows - 1) / kGradRows * kGradRows;
   return {(int)range, (int)((M + range - 1) / range)};
 }
 
@@ -555,7 +577,7 @@ extern "C" int kda_lora_grad(int64_t M, int32_t J, int32_t R, int32_t n, const i
   int rc = kda::check_lora("lora_grad", M, J, R, n, ids, rows_per_id);
   if (rc != KDA_OK) return rc;
   KDA_REQUIRE(grad && aligned16(grad), "lora_grad: null or unaligned pointer");
-  GradPlan p{32, 0};
+  GradPlan p{kGradRows, 0};
   float* part = (float*)scratch;
   int32_t* flag = nullptr;
   if (M > 0) {

@@ -21,17 +21,16 @@ constexpr int kGlThreads = (kGlCompute + 2) * kWave;
 constexpr int kGlPart = kGlTile * kGlDepth * 2;  // 8 KB: one operand's step
 constexpr int kGlStage = 2 * kGlPart;
 constexpr int kGlLoads = kGlPart / 1024;         // loads of a step and loader
-constexpr int kGlAdPitch = 64 + 4;               // a wave's 32 x 64 piece of F (WT)
+constexpr int kGlPiecePitch = 32 + 8;            // a wave's 32 x 32 piece of F (WT)
 static_assert(64 * 128 <= kGlStage / 2, "a wave's 64 x 64 results fit half a stage");
 static_assert((kGlStages - 2) * kGlLoads < 64, "vmcnt range");
-static_assert(32 * kGlAdPitch * 2 <= kGlStage / 2, "a wave's piece of F fits half a stage");
 
 // A step of a row-major operand whose rows run along the contraction: 128 rows of 64 bytes.  The
-// 16-byte chunk c of row r sits in slot c ^ (r / 2 % 4), so that eight neighbouring rows' reads of
+// 16-byte chunk c of row r sits in slot c ^ (r / 4 % 4), so that sixteen neighbouring rows' reads of
 // one chunk fall on different banks.
 __device__ __forceinline__ bf16x8 gl_row_frag(const char* part, int r0, int lane) {
   const int r = r0 + lane % 16;
-  return *reinterpret_cast<const bf16x8*>(part + r * 64 + (((lane / 16) ^ (r >> 1 & 3)) << 4));
+  return *reinterpret_cast<const bf16x8*>(part + r * 64 + (((lane / 16) ^ (r >> 2 & 3)) << 4));
 }
 // A step of an operand whose rows are the contraction's: 32 rows of 256 bytes, chunk c of row r in
 // slot c ^ (2 (r % 4)); fragments run down the columns (two transposing reads).
@@ -51,6 +50,7 @@ __global__ __launch_bounds__(kGlThreads, 3) void lora_linear_kernel(LoraRows row
                                                                     const bf16* __restrict__ f, bf16* __restrict__ y,
                                                                     int tiles_n, int items) {
   __shared__ __attribute__((aligned(16))) char smem[kGlStages * kGlStage];
+  __shared__ __attribute__((aligned(16))) bf16 piece[WT ? kGlCompute : 1][WT ? 32 * kGlPiecePitch : 1];
   const int per_xcd = (items + kXcds - 1) / kXcds;
   const int item = (blockIdx.x % kXcds) * per_xcd + blockIdx.x / kXcds;
   if (blockIdx.x / kXcds >= per_xcd || item >= items) return;  // grid rounding (the whole workgroup)
@@ -60,31 +60,41 @@ __global__ __launch_bounds__(kGlThreads, 3) void lora_linear_kernel(LoraRows row
   constexpr int P = kGlStages - 1;
 
   if (wave >= kGlCompute) {
-    // ---- loader waves: wave 4 moves rows of x, wave 5 W ----
+    // ---- loader waves: wave 4 moves rows of x, wave 5 W.  A step is kGlLoads loads whose offsets from the
+    // step's base do not change (kDropOffset: outside the operand), so that issuing one keeps up with
+    // the products; only the last step may have columns to drop ----
     const bool isx = wave == kGlCompute;
+    const bool cols = WT && !isx;  // rows of the contraction
+    const long ld = cols ? N : isx ? ldx : (long)K;
+    int off[kGlLoads], k_of[kGlLoads];  // byte offset and place in the step's 32 of the contraction
+#pragma unroll
+    for (int i = 0; i < kGlLoads; ++i) {
+      if (cols) {
+        const int r = 4 * i + lane / 16, c = 8 * ((lane % 16) ^ (2 * (r & 3)));
+        k_of[i] = r;
+        off[i] = n0 + c < N ? (r * N + c) * 2 : kDropOffset;
+      } else {
+        const int r = 16 * i + lane / 4, k = 8 * ((lane % 4) ^ (r >> 2 & 3));
+        k_of[i] = k;
+        off[i] = (isx ? m0 + r < rows.M : n0 + r < N) ? (int)(r * ld + k) * 2 : kDropOffset;
+      }
+    }
+    const bf16* base = cols ? w + n0 : (isx ? x + (size_t)m0 * ldx : w + (size_t)n0 * K);
+    const size_t advance = cols ? (size_t)kGlDepth * N : kGlDepth;
     auto issue = [&](int q) {
       char* st = smem + (q % kGlStages) * kGlStage + (isx ? 0 : kGlPart);
-      const int k0 = kGlDepth * q;
-      if (WT && !isx) {
-        const __amdgpu_buffer_rsrc_t rs = raw_rsrc(w + (size_t)k0 * N + n0);
+      const __amdgpu_buffer_rsrc_t rs = raw_rsrc(base + q * advance);
+      const int left = K - kGlDepth * q;
+      if (left >= kGlDepth) {
 #pragma unroll
-        for (int i = 0; i < kGlLoads; ++i) {
-          const int r = 4 * i + lane / 16, c = 8 * ((lane % 16) ^ (2 * (r & 3)));
-          const bool ok = k0 + r < K && n0 + c < N;
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(st + i * 1024), 16,
-                                                   ok ? (r * N + c) * 2 : kDropOffset, 0, 0, 0);
-        }
+        for (int i = 0; i < kGlLoads; ++i)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(st + i * 1024), 16, off[i],
+                                                   0, 0, 0);
       } else {
-        const long ld = isx ? ldx : (long)K;
-        const int r0 = isx ? m0 : n0, rn = isx ? rows.M : N;
-        const __amdgpu_buffer_rsrc_t rs = raw_rsrc((isx ? x : w) + (size_t)r0 * ld);
 #pragma unroll
-        for (int i = 0; i < kGlLoads; ++i) {
-          const int r = 16 * i + lane / 4, k = k0 + 8 * ((lane % 4) ^ (r >> 1 & 3));
-          const bool ok = r0 + r < rn && k < K;
+        for (int i = 0; i < kGlLoads; ++i)
           __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(st + i * 1024), 16,
-                                                   ok ? (int)((r * ld + k) * 2) : kDropOffset, 0, 0, 0);
-        }
+                                                   k_of[i] < left ? off[i] : kDropOffset, 0, 0, 0);
       }
     };
     auto wait_landed = [&](int later) {  // all but the last `later` steps issued have landed
@@ -99,7 +109,7 @@ __global__ __launch_bounds__(kGlThreads, 3) void lora_linear_kernel(LoraRows row
     ring_barrier();  // B0: step 0 visible
     for (int q = 0; q < nsteps; ++q) {
       wait_landed(max(0, min(P - 2, nsteps - 2 - q)));
-      ring_barrier();  // A(q): step q + 1 visible; step q's slot is free
+      ring_barrier();  // A(q): step q + 1 visible; step q - 1's slot is read
       if (q + P < nsteps) issue(q + P);
     }
     return;
@@ -107,11 +117,71 @@ __global__ __launch_bounds__(kGlThreads, 3) void lora_linear_kernel(LoraRows row
 
   // ---- compute wave (wm, wn): rows m0 + 64 wm .., columns n0 + 64 wn .. ----
   const int wm = wave / 2, wn = wave % 2, lr = lane % 16, kg = lane / 16;
+  const int mw = m0 + 64 * wm, nw = n0 + 64 * wn;
   f32x4 acc[4][4];  // [column tile][row tile]
 #pragma unroll
   for (int c = 0; c < 4; ++c)
 #pragma unroll
     for (int t = 0; t < 4; ++t) acc[c][t] = zero4();
+
+  // ---- first, while the loaders' first steps are on their way, the adapters of the wave's 64 rows, one
+  // after another ----
+  {
+    const int row_id = rows.id(mw + lane);
+    const size_t plane = (size_t)rows.M * R;
+    // (buffers from the wave's first row or column: 32-bit offsets, and what is outside reads as zero)
+    const __amdgpu_buffer_rsrc_t rhi = raw_rsrc(u + (size_t)mw * R), rlo = raw_rsrc(u + plane + (size_t)mw * R);
+    int a = next_adapter(row_id, -1), r0 = 0;
+    while (a != kNoAdapter) {
+      const int r = r0 + 8 * kg;
+      const size_t base = (size_t)a * R * N;
+      bf16x8 ff[4];
+      if constexpr (WT) {
+        const __amdgpu_buffer_rsrc_t rf = raw_rsrc(f + base + (size_t)r0 * N + nw);
+        const int rr = lane / 4, c = 8 * (lane % 4);
+        bf16x8 v[2][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)  // 32 rows of 32 columns
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            v[h][i] = buffer8(rf, r0 + 16 * i + rr < R && nw + 32 * h + c < N ? (rr * N + c) * 2 : kDropOffset, 32 * i * N + 64 * h);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          asm volatile("" ::: "memory");
+#pragma unroll
+          for (int i = 0; i < 2; ++i) *(bf16x8*)(piece[wave] + (16 * i + rr) * kGlPiecePitch + c) = v[h][i];
+          asm volatile("" ::: "memory");
+#pragma unroll
+          for (int c2 = 0; c2 < 2; ++c2) ff[2 * h + c2] = lds_col_frag(piece[wave], kGlPiecePitch, 0, 16 * c2, lane);
+        }
+      } else {
+        const __amdgpu_buffer_rsrc_t rf = raw_rsrc(f + base + (size_t)nw * R);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          ff[c] = buffer8(rf, r < R && nw + 16 * c + lr < N ? (lr * R + r) * 2 : kDropOffset, 32 * c * R);
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const bool mine = __shfl(row_id, 16 * t + lr) == a;
+        const int off = r < R && mw + 16 * t + lr < rows.M ? (lr * R + r) * 2 : kDropOffset;
+        const bf16x8 hi = buffer8(rhi, off, 32 * t * R), lo = buffer8(rlo, off, 32 * t * R);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          // (chosen, not multiplied by zero: an infinity in this adapter stays out of other rows)
+          const f32x4 d = mfma16(ff[c], lo, mfma16(ff[c], hi, zero4()));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[c][t][i] += mine ? d[i] : 0.f;
+        }
+        __builtin_amdgcn_sched_barrier(0);  // (all rows at once would spill registers)
+      }
+      r0 += kGlDepth;
+      if (r0 >= R) {
+        r0 = 0;
+        a = next_adapter(row_id, a);
+      }
+    }
+  }
+
   ring_barrier();  // B0
   for (int q = 0; q < nsteps; ++q) {
     const char* st = smem + (q % kGlStages) * kGlStage;
@@ -128,68 +198,10 @@ __global__ __launch_bounds__(kGlThreads, 3) void lora_linear_kernel(LoraRows row
     ring_barrier();  // A(q)
   }
 
-  // ---- the adapters of the wave's 64 rows, one after another ----
-  const int mw = m0 + 64 * wm, nw = n0 + 64 * wn;
-  const int row_id = rows.id(mw + lane);
-  const size_t plane = (size_t)rows.M * R;
-  // (buffers from the wave's first row or column: 32-bit offsets, and what is outside reads as zero)
-  const __amdgpu_buffer_rsrc_t rhi = raw_rsrc(u + (size_t)mw * R), rlo = raw_rsrc(u + plane + (size_t)mw * R);
-  // half a stage per wave, of stages that nobody reads any more (the last step's is not among them):
-  // pieces of F (WT), and the result
-  bf16* piece = reinterpret_cast<bf16*>(smem + ((nsteps + wave / 2) % kGlStages) * kGlStage + (wave % 2) * (kGlStage / 2));
-  // one loop over adapters and their 32-deep steps, entered in any case (without an adapter nothing is
-  // read and no row takes the result): a loop behind a branch doubled the accumulators' registers
-  int a = next_adapter(row_id, -1), r0 = 0;
-  do {
-    const int r = a == kNoAdapter ? R : r0 + 8 * kg;
-    const size_t base = a == kNoAdapter ? 0 : (size_t)a * R * N;
-    bf16x8 ff[4];
-    if constexpr (WT) {
-      const __amdgpu_buffer_rsrc_t rf = raw_rsrc(f + base + (size_t)r0 * N + nw);
-      const int rr = lane / 8, c = 8 * (lane % 8);
-      uint4 v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)  // 32 rows of 64 columns: 8 of 16 bytes each
-        v[i] = __builtin_bit_cast(uint4, buffer8(rf, a != kNoAdapter && r0 + 8 * i + rr < R && nw + c < N ? (rr * N + c) * 2 : kDropOffset, 16 * i * N));
-      asm volatile("" ::: "memory");
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint2* d = (uint2*)(piece + (8 * i + rr) * kGlAdPitch + c);
-        d[0] = make_uint2(v[i].x, v[i].y);
-        d[1] = make_uint2(v[i].z, v[i].w);
-      }
-      asm volatile("" ::: "memory");
-#pragma unroll
-      for (int c = 0; c < 4; ++c) ff[c] = lds_col_frag(piece, kGlAdPitch, 0, 16 * c, lane);
-    } else {
-      const __amdgpu_buffer_rsrc_t rf = raw_rsrc(f + base + (size_t)nw * R);
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        ff[c] = buffer8(rf, r < R && nw + 16 * c + lr < N ? (lr * R + r) * 2 : kDropOffset, 32 * c * R);
-    }
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const bool mine = __shfl(row_id, 16 * t + lr) == a;
-      const int off = r < R && mw + 16 * t + lr < rows.M ? (lr * R + r) * 2 : kDropOffset;
-      const bf16x8 hi = buffer8(rhi, off, 32 * t * R), lo = buffer8(rlo, off, 32 * t * R);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        // (chosen, not multiplied by zero: an infinity in this adapter stays out of other rows)
-        const f32x4 d = mfma16(ff[c], lo, mfma16(ff[c], hi, zero4()));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[c][t][i] += mine ? d[i] : 0.f;
-      }
-      __builtin_amdgcn_sched_barrier(0);  // (all rows at once would spill registers)
-    }
-    r0 += kGlDepth;
-    if (r0 >= R) {
-      r0 = 0;
-      a = next_adapter(row_id, a);
-    }
-  } while (a != kNoAdapter);
   // accumulator: column 16 c + 4 kg + i, row 16 t + lr of the wave's 64; through the wave's half stage
-  // (128-byte rows, chunk q of row r in slot q ^ (r % 8)), so that eight lanes store a row's line
-  char* out = reinterpret_cast<char*>(piece);
+  // (128-byte rows, chunk q of row r in slot q ^ (r % 8); of stages that nobody reads any more: the last
+  // step's is not among them), so that eight lanes store a row's line
+  char* out = smem + ((nsteps + wave / 2) % kGlStages) * kGlStage + (wave % 2) * (kGlStage / 2);
   asm volatile("" ::: "memory");
 #pragma unroll
   for (int t = 0; t < 4; ++t)
@@ -232,4 +244,43 @@ extern "C" int kda_lora_linear(int64_t M, int32_t N, int32_t K, int32_t R, int32
   weight_rows ? go(lora_linear_kernel<true>) : go(lora_linear_kernel<false>);
   KDA_LAUNCH_CHECK("lora_linear");
   return KDA_OK;
+}
+
+extern "C" int kda_lora_forward(int64_t M, int32_t N, int32_t K, int32_t R, int32_t n, const int32_t* ids,
+                                int64_t rows_per_id, const void* x, int64_t ldx, const void* weight,
+                                const void* lora_a, const void* lora_b, const float* scale, int32_t how, void* u,
+                                void* y, hipStream_t stream) {
+  KDA_REQUIRE(how >= KDA_LORA_ROWS && how <= KDA_LORA_PART, "lora_forward: unknown way");
+  if (how == KDA_LORA_ROWS) {
+    KDA_REQUIRE(M >= 0 && M <= 64, "lora_forward: at most 64 rows");
+    return kda_lora_linear_rows((int32_t)M, N, K, R, n, ids, rows_per_id, x, ldx, weight, lora_a, lora_b, scale, u, y,
+                                stream);
+  }
+  int rc = kda_lora_shrink(M, K, R, n, ids, rows_per_id, x, ldx, lora_a, 0, scale, u, stream);
+  if (rc != KDA_OK) return rc;
+  if (how == KDA_LORA_WHOLE)
+    return kda_lora_linear(M, N, K, R, n, ids, rows_per_id, x, ldx, weight, 0, u, lora_b, y, stream);
+  return kda_lora_expand(M, N, R, n, ids, rows_per_id, u, lora_b, 1, y, N, stream);
+}
+
+extern "C" size_t kda_lora_backward_scratch_bytes(int64_t M, int32_t N, int32_t K, int32_t R, int32_t n) {
+  const size_t a = kda_lora_grad_scratch_bytes(M, K, R, n), b = kda_lora_grad_scratch_bytes(M, N, R, n);
+  return a > b ? a : b;
+}
+
+extern "C" int kda_lora_backward(int64_t M, int32_t N, int32_t K, int32_t R, int32_t n, const int32_t* ids,
+                                 int64_t rows_per_id, const void* x, int64_t ldx, const void* grad_output, int64_t ldg,
+                                 const void* weight, const void* lora_a, const void* lora_b, const float* scale,
+                                 const void* u, int32_t how, void* t, void* dx, float* da, float* db, void* scratch,
+                                 hipStream_t stream) {
+  KDA_REQUIRE(how == KDA_LORA_WHOLE || how == KDA_LORA_PART, "lora_backward: unknown way");
+  int rc = KDA_OK;
+  if (dx || da) rc = kda_lora_shrink(M, N, R, n, ids, rows_per_id, grad_output, ldg, lora_b, 1, scale, t, stream);
+  if (rc == KDA_OK && dx)
+    rc = how == KDA_LORA_WHOLE
+             ? kda_lora_linear(M, K, N, R, n, ids, rows_per_id, grad_output, ldg, weight, 1, t, lora_a, dx, stream)
+             : kda_lora_expand(M, K, R, n, ids, rows_per_id, t, lora_a, 0, dx, K, stream);
+  if (rc == KDA_OK && da) rc = kda_lora_grad(M, K, R, n, ids, rows_per_id, x, ldx, t, 0, da, scratch, stream);
+  if (rc == KDA_OK && db) rc = kda_lora_grad(M, N, R, n, ids, rows_per_id, grad_output, ldg, u, 1, db, scratch, stream);
+  return rc;
 }

@@ -214,18 +214,6 @@ def linear_few_rows(m, x, *, relu2=False, residual=None):
     return ops.linear_rows(x, w16, relu2=relu2, residual=residual)
 
 
-def _lora_forward(x2, w16, a16, b16, ids, scaling):
-    """(y, u) = (x W^T + u B_a^T, s_a x A_a^T) of the rows x2 [M, K], a the row's adapter.  One rounding of
-    y, or for the long contractions that the library multiplies two of the adapters' part, which is
-    then formed first and the shared projection added to it."""
-    if ops.lora_linear_rows_fits(x2, w16):
-        return ops.lora_linear_rows(x2, w16, a16, b16, ids, scaling)
-    u = ops.lora_shrink(x2, a16, ids, scaling)
-    if ops.lora_linear_gains(x2.shape[0], x2.shape[1], w16.shape[0]):
-        return ops.lora_linear(x2, w16, u, b16, ids), u
-    return ops.lora_expand(u, b16, ids, factor_cols=True).addmm_(x2, w16.t()), u
-
-
 class _LoraLinear(torch.autograd.Function):
     """A projection with adapters, for autograd: bf16 W, A and B (casts of the masters, whose gradients
     come back in f32)."""
@@ -233,7 +221,7 @@ class _LoraLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, a, b, ids, scaling, w16, a16, b16):
         x2 = x.reshape(-1, x.shape[-1])
-        y, u = _lora_forward(x2, w16, a16, b16, ids, scaling)
+        y, u = ops.lora_forward(x2, w16, a16, b16, ids, scaling)
         ctx.save_for_backward(x2, w16, a16, b16, ids, scaling, u)
         ctx.shape, ctx.types = x.shape, (weight.dtype, a.dtype, b.dtype)
         return y.view(*x.shape[:-1], w16.shape[0])
@@ -244,22 +232,22 @@ class _LoraLinear(torch.autograd.Function):
         x2, w16, a16, b16, ids, scaling, u = ctx.saved_tensors
         need = ctx.needs_input_grad
         g2 = grad.reshape(-1, grad.shape[-1]).to(torch.bfloat16)
-        dx = dw = da = db = None
-        if need[0] or need[2]:
-            t = ops.lora_shrink(g2, b16, ids, scaling, factor_cols=True)
-            if need[0]:
-                if ops.lora_linear_gains(*g2.shape, w16.shape[1]):
-                    dx = ops.lora_linear(g2, w16, t, a16, ids, weight_rows=True)
-                else:
-                    dx = ops.lora_expand(t, a16, ids).addmm_(g2, w16)
-                dx = dx.view(ctx.shape)
-            if need[2]:
-                da = ops.lora_grad(x2, t, ids, a16.shape[0]).to(ctx.types[1])
+        dx, da, db = ops.lora_backward(x2, w16, a16, b16, ids, scaling, u, g2, need[0], need[2], need[3])
+        dw = None
         if need[1]:
             dw = (ops.weight_grad(g2, x2) if w16.numel() <= _SPLIT_WGRAD_MAX else _mm_f32(g2.t(), x2)).to(ctx.types[0])
-        if need[3]:
-            db = ops.lora_grad(g2, u, ids, b16.shape[0], out_cols=True).to(ctx.types[2])
-        return dx, dw, da, db, None, None, None, None, None
+        return (dx.view(ctx.shape) if need[0] else None, dw, da.to(ctx.types[1]) if need[2] else None,
+                db.to(ctx.types[2]) if need[3] else None, None, None, None, None, None)
+
+
+def _cast16(*tensors):
+    """bf16 values of the tensors; f32 masters that lie as one launch takes them cast in one."""
+    if all(t.dtype == torch.float32 and t.is_contiguous() and t.numel() % 8 == 0 and t.numel() and t.data_ptr() % 16 == 0
+           and t.device == tensors[0].device for t in tensors):
+        counts = [t.numel() for t in tensors]
+        parts = torch.split(ops.cast_weights_bf16([t.detach() for t in tensors], counts), counts)
+        return [p.view(t.shape) for p, t in zip(parts, tensors)]
+    return [t if t.dtype == torch.bfloat16 else t.detach().to(torch.bfloat16) for t in tensors]
 
 
 def _lora_linear(x, weight, a, b, ids, scaling, w16, a16, b16):
@@ -268,7 +256,7 @@ def _lora_linear(x, weight, a, b, ids, scaling, w16, a16, b16):
     ids = ids if ids.is_contiguous() else ids.contiguous()
     scaling = scaling if scaling.dtype == torch.float32 else scaling.detach().float()
     if not _needs_grad(x, weight, a, b) and _untransformed(x, weight, a, b, ids, scaling):
-        y, _ = _lora_forward(x.reshape(-1, x.shape[-1]), w16, a16, b16, ids, scaling)
+        y, _ = ops.lora_forward(x.reshape(-1, x.shape[-1]), w16, a16, b16, ids, scaling)
         return y.view(*x.shape[:-1], w16.shape[0])
     return _LoraLinear.apply(x, weight, a, b, ids, scaling, w16, a16, b16)
 
@@ -299,8 +287,8 @@ def lora_linear(x, weight, lora_a, lora_b, adapter_ids, scaling):
     types; scaling is a constant."""
     ids = _check_lora(x, weight, lora_a, lora_b, adapter_ids, scaling)
     if x.is_cuda and x.dtype == torch.bfloat16:
-        w16, a16, b16 = [t if t.dtype == torch.bfloat16 else t.detach().to(torch.bfloat16) for t in (weight, lora_a, lora_b)]
-        return _lora_linear(x, weight, lora_a, lora_b, ids, scaling, w16, a16, b16)
+        w16 = weight if weight.dtype == torch.bfloat16 else weight.detach().to(torch.bfloat16)
+        return _lora_linear(x, weight, lora_a, lora_b, ids, scaling, w16, *_cast16(lora_a, lora_b))
     return _lora_eager(x, weight, lora_a, lora_b, ids, scaling)
 
 
@@ -343,7 +331,7 @@ class LoraLinear(Linear):
                             self.weight.detach().to(torch.bfloat16) if w16 is None else w16, a16, b16)
 
     def adapters_bf16(self):
-        return tuple(t.detach().to(torch.bfloat16) for t in (self.lora_a, self.lora_b))
+        return tuple(_cast16(self.lora_a, self.lora_b))
 
 
 def _norm_gate_eager(x, gate, weight, eps):

@@ -17,7 +17,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import ChunkProblem, KDA_GATE_K3, KDA_GATE_LOGDECAY, check, ptr
+from ._lib import ChunkProblem, KDA_GATE_K3, KDA_GATE_LOGDECAY, KDA_LORA_PART, KDA_LORA_ROWS, KDA_LORA_WHOLE, check, ptr
 
 GATE_MODES = {"k3": KDA_GATE_K3, "precomputed": KDA_GATE_LOGDECAY}
 
@@ -808,132 +808,76 @@ def embedding_backward(idx, grad_output, vocab):
     return dw
 
 
-def _lora_rows(what, ids, rows):
-    """Rows for each entry of ids: 1 (an id a row) or as many as a sequence has."""
-    if ids.dtype != torch.int32 or not ids.is_contiguous() or (rows and (ids.numel() == 0 or rows % ids.numel())):
-        raise RuntimeError(f"{what}: contiguous int32 ids expected, each for the same number of rows")
-    return rows // ids.numel() if rows else 1
+def _lora_way(M, K, N):
+    """How a contraction of K with its adapters runs best on M rows and N outputs: as one kernel, or the
+    adapters' part alone with a library product added to it.  One kernel takes 22 us against 43 for M 8192,
+    K 384, N 1536, 20 / 28 for 8192 x 768 x 768, 9 / 18 for 2048 x 384 x 1536, 22 / 27 for 8192 x 1536 x 384,
+    but 20 / 17 for 2048 x 1536 x 384 (48 tiles), 105 / 84 for 8192 x 1024 x 4096 and 165 / 111 for 7777 x
+    4096 x 2048 (the library's larger tiles)."""
+    whole = K <= 768 or (K <= 1536 and N <= 1024 and -(-M // 128) * -(-N // 128) >= 128)
+    return KDA_LORA_WHOLE if whole else KDA_LORA_PART
 
 
-def lora_shrink(x, factor, ids, scale, *, factor_cols=False):
-    """u = scale[a] F_a x of the rows x [M, J] bf16, a = the row's adapter (ids: one a row, or one for every
-    M / numel rows; outside [0, n): zeros), as three bf16 parts [3, M, R] whose sum is the f32 value.
-    factor [n, R, J] bf16, with ``factor_cols`` [n, J, R]; scale [n] f32 or None."""
-    what = "lora_shrink"
-    dev = _require_cuda(what, x, factor, ids, scale)
-    _check_dtype(what, x, torch.bfloat16, "x")
-    _check_dtype(what, factor, torch.bfloat16, "factor")
-    _check_dtype(what, scale, torch.float32, "scale")
-    if x.ndim != 2 or factor.ndim != 3 or factor.shape[1 if factor_cols else 2] != x.shape[1]:
-        raise RuntimeError(f"{what}: x [M, J] and factor [n, R, J] (factor_cols: [n, J, R]) expected")
-    n, R, J = factor.shape[0], factor.shape[2 if factor_cols else 1], x.shape[1]
-    if scale is not None and scale.shape != (n,):
-        raise RuntimeError(f"{what}: scale must have shape {(n,)}")
-    per = _lora_rows(what, ids, x.shape[0])
-    x, factor, scale = _c(x), _c(factor), _c(scale)
-    u = torch.empty(3, x.shape[0], R, dtype=torch.bfloat16, device=dev)
-    with _on(dev):
-        rc = _lib.load().kda_lora_shrink(x.shape[0], J, R, n, ptr(ids), per, ptr(x), J, ptr(factor),
-                                         1 if factor_cols else 0, ptr(scale), ptr(u), _stream(dev))
-    check(rc, "kda_lora_shrink")
-    return u
-
-
-def lora_expand(u, factor, ids, *, factor_cols=False):
-    """y [M, J] bf16 = F_a^T u of the rows u [3, M, R]; factor and ids as in :func:`lora_shrink`."""
-    what = "lora_expand"
-    dev = _require_cuda(what, u, factor, ids)
-    _check_dtype(what, u, torch.bfloat16, "u")
-    _check_dtype(what, factor, torch.bfloat16, "factor")
-    if u.ndim != 3 or u.shape[0] != 3 or factor.ndim != 3 or factor.shape[2 if factor_cols else 1] != u.shape[2]:
-        raise RuntimeError(f"{what}: u [3, M, R] and factor [n, R, J] (factor_cols: [n, J, R]) expected")
-    n, J, M, R = factor.shape[0], factor.shape[1 if factor_cols else 2], u.shape[1], u.shape[2]
-    per = _lora_rows(what, ids, M)
-    u, factor = _c(u), _c(factor)
-    y = torch.empty(M, J, dtype=torch.bfloat16, device=dev)
-    with _on(dev):
-        rc = _lib.load().kda_lora_expand(M, J, R, n, ptr(ids), per, ptr(u), ptr(factor),
-                                         1 if factor_cols else 0, ptr(y), J, _stream(dev))
-    check(rc, "kda_lora_expand")
-    return y
-
-
-def lora_linear(x, w16, u, factor, ids, *, weight_rows=False):
-    """y [M, N] bf16 = x W^T + u B_a of the rows x [M, K] (w16 [N, K], factor [n, N, R]), u [3, M, R] from
-    :func:`lora_shrink`; ``weight_rows``: x W + u F_a with w16 [K, N], factor [n, R, N].  One rounding."""
-    what = "lora_linear"
-    dev = _require_cuda(what, x, w16, u, factor, ids)
-    for name, t in (("x", x), ("w16", w16), ("u", u), ("factor", factor)):
-        _check_dtype(what, t, torch.bfloat16, name)
-    (M, K), R, n = x.shape, u.shape[2], factor.shape[0]
-    N = w16.shape[1 if weight_rows else 0]
-    if w16.shape != ((K, N) if weight_rows else (N, K)) or u.shape != (3, M, R) or factor.shape != ((n, R, N) if weight_rows else (n, N, R)):
-        raise RuntimeError(f"{what}: x [M, K], w16 [N, K], u [3, M, R], factor [n, N, R] (weight_rows: [K, N], [n, R, N]) expected")
-    per = _lora_rows(what, ids, M)
-    x, w16, u, factor = _c(x), _c(w16), _c(u), _c(factor)
-    y = torch.empty(M, N, dtype=torch.bfloat16, device=dev)
-    with _on(dev):
-        rc = _lib.load().kda_lora_linear(M, N, K, R, n, ptr(ids), per, ptr(x), K, ptr(w16), 1 if weight_rows else 0,
-                                         ptr(u), ptr(factor), ptr(y), _stream(dev))
-    check(rc, "kda_lora_linear")
-    return y
-
-
-def lora_linear_gains(M, K, N):
-    """Whether :func:`lora_linear` beats :func:`lora_expand` and a library product added to it, on M rows
-    and a contraction of K: M 8192, K 384, N 1536 25 us against 49, 8192 x 768 x 768 22 / 33, 2048 x 384 x
-    1536 10 / 20, 8192 x 1536 x 384 23 / 30, but 2048 x 1536 x 384 (48 tiles) 21 / 18, 8192 x 1024 x 4096
-    111 / 93, 7777 x 4096 x 2048 162 / 121 (the library's larger tiles)."""
-    return K <= 768 or (K <= 1536 and N <= 1024 and -(-M // 128) * -(-N // 128) >= 128)
-
-
-def lora_linear_rows_fits(x, w16):
-    """Whether :func:`lora_linear_rows` takes the rows x [M, K] with weight w16 [N, K]."""
-    return 0 < x.shape[0] <= _LINEAR_ROWS and x.shape[1] % 32 == 0 and w16.shape[0] % 4 == 0
-
-
-def lora_linear_rows(x, w16, a, b, ids, scale):
-    """(x W^T + scale_a (x A_a^T) B_a^T bf16, u) of at most 64 rows x [M, K]; a [n, R, K], b [n, N, R], and
-    ids, scale and u as in :func:`lora_shrink`.  Two launches, one rounding."""
-    what = "lora_linear_rows"
+def _lora_check(what, x, w16, a, b, ids, scale):
     dev = _require_cuda(what, x, w16, a, b, ids, scale)
     for name, t in (("x", x), ("w16", w16), ("a", a), ("b", b)):
         _check_dtype(what, t, torch.bfloat16, name)
     _check_dtype(what, scale, torch.float32, "scale")
-    (M, K), (n, R), N = x.shape, a.shape[:2], w16.shape[0]
-    if not lora_linear_rows_fits(x, w16) or w16.shape[1] != K or a.shape[2] != K or b.shape != (n, N, R) or scale.shape != (n,):
-        raise RuntimeError(f"{what}: x [M, K] of at most 64 rows, w16 [N, K], a [n, R, K], b [n, N, R], scale [n] expected")
-    per = _lora_rows(what, ids, M)
+    _check_dtype(what, ids, torch.int32, "ids")
+    if x.ndim != 2 or w16.ndim != 2 or a.ndim != 3 or w16.shape[1] != x.shape[1] or a.shape[2] != x.shape[1] or \
+            b.shape != (a.shape[0], w16.shape[0], a.shape[1]) or scale.shape != a.shape[:1]:
+        raise RuntimeError(f"{what}: x [M, K], w16 [N, K], a [n, R, K], b [n, N, R] and scale [n] expected")
+    rows = x.shape[0]
+    if not ids.is_contiguous() or (rows and (ids.numel() == 0 or rows % ids.numel())):
+        raise RuntimeError(f"{what}: contiguous ids expected, each for the same number of rows")
+    return dev, (rows // ids.numel() if rows else 1)
+
+
+def lora_forward(x, w16, a, b, ids, scale):
+    """(y, u): y = x W^T + u B_a^T of the rows x [M, K] bf16 with a = the row's adapter (ids int32: one a row,
+    or one for every M / numel rows; outside [0, n): none), w16 [N, K], a [n, R, K], b [n, N, R] bf16, scale
+    [n] f32.  u [3, M, R] = scale_a x A_a^T as three bf16 parts whose sum is the f32 value.  y is rounded
+    once; where the library multiplies x W^T (:func:`_lora_way`), the adapters' part once before."""
+    dev, per = _lora_check("lora_forward", x, w16, a, b, ids, scale)
     x, w16, a, b, scale = _c(x), _c(w16), _c(a), _c(b), _c(scale)
+    (M, K), N, (n, R) = x.shape, w16.shape[0], a.shape[:2]
     u = torch.empty(3, M, R, dtype=torch.bfloat16, device=dev)
     y = torch.empty(M, N, dtype=torch.bfloat16, device=dev)
+    how = KDA_LORA_ROWS if M <= _LINEAR_ROWS and K % 32 == 0 else _lora_way(M, K, N)
     with _on(dev):
-        rc = _lib.load().kda_lora_linear_rows(M, N, K, R, n, ptr(ids), per, ptr(x), K, ptr(w16), ptr(a), ptr(b),
-                                              ptr(scale), ptr(u), ptr(y), _stream(dev))
-    check(rc, "kda_lora_linear_rows")
+        rc = _lib.load().kda_lora_forward(M, N, K, R, n, ptr(ids), per, ptr(x), K, ptr(w16), ptr(a), ptr(b), ptr(scale),
+                                          how, ptr(u), ptr(y), _stream(dev))
+        check(rc, "kda_lora_forward")
+        if how == KDA_LORA_PART:
+            y.addmm_(x, w16.t())
     return y, u
 
 
-def lora_grad(x, u, ids, n, *, out_cols=False):
-    """G [n, R, J] f32 (``out_cols``: [n, J, R]), G_a = sum over adapter a's rows of u [3, M, R]
-    times x [M, J] bf16; ids and u as in :func:`lora_shrink`.  Fixed-order sums."""
-    what = "lora_grad"
-    dev = _require_cuda(what, x, u, ids)
-    _check_dtype(what, x, torch.bfloat16, "x")
-    _check_dtype(what, u, torch.bfloat16, "u")
-    if x.ndim != 2 or u.ndim != 3 or u.shape[:2] != (3, x.shape[0]):
-        raise RuntimeError(f"{what}: x [M, J] and u [3, M, R] expected")
-    (M, J), R = x.shape, u.shape[2]
-    per = _lora_rows(what, ids, M)
-    x, u = _c(x), _c(u)
+def lora_backward(x, w16, a, b, ids, scale, u, grad, need_x, need_a, need_b):
+    """(dx [M, K] bf16, da [n, R, K] f32, db [n, N, R] f32) of :func:`lora_forward` for grad [M, N] bf16, those
+    that are needed (else None); fixed-order sums.  Adapters without rows get zeros."""
+    what = "lora_backward"
+    dev, per = _lora_check(what, x, w16, a, b, ids, scale)
+    _check_dtype(what, grad, torch.bfloat16, "grad")
+    (M, K), N, (n, R) = x.shape, w16.shape[0], a.shape[:2]
+    if grad.shape != (M, N) or u.shape != (3, M, R) or u.dtype != torch.bfloat16 or {grad.device, u.device} != {dev}:
+        raise RuntimeError(f"{what}: grad [M, N] and u [3, M, R] expected")
+    x, w16, a, b, scale, u, grad = (_c(t) for t in (x, w16, a, b, scale, u, grad))
     lib = _lib.load()
-    scratch = torch.empty(lib.kda_lora_grad_scratch_bytes(M, J, R, n), dtype=torch.uint8, device=dev)
-    grad = torch.empty((n, J, R) if out_cols else (n, R, J), dtype=torch.float32, device=dev)
+    how = _lora_way(M, N, K)
+    t = torch.empty_like(u) if need_x or need_a else None
+    dx = torch.empty_like(x) if need_x else None
+    da = torch.empty(n, R, K, dtype=torch.float32, device=dev) if need_a else None
+    db = torch.empty(n, N, R, dtype=torch.float32, device=dev) if need_b else None
+    scratch = torch.empty(lib.kda_lora_backward_scratch_bytes(M, N, K, R, n), dtype=torch.uint8, device=dev)
     with _on(dev):
-        rc = lib.kda_lora_grad(M, J, R, n, ptr(ids), per, ptr(x), J, ptr(u), 1 if out_cols else 0, ptr(grad),
-                               ptr(scratch), _stream(dev))
-    check(rc, "kda_lora_grad")
-    return grad
+        rc = lib.kda_lora_backward(M, N, K, R, n, ptr(ids), per, ptr(x), K, ptr(grad), N, ptr(w16), ptr(a), ptr(b),
+                                   ptr(scale), ptr(u), how, ptr(t), ptr(dx), ptr(da), ptr(db), ptr(scratch),
+                                   _stream(dev))
+        check(rc, "kda_lora_backward")
+        if need_x and how == KDA_LORA_PART:
+            dx.addmm_(grad, w16)
+    return dx, da, db
 
 
 def softcap_cross_entropy_backward(logits, targets, lse, grad_scale, vocab, softcap, ignore_index=-1):

@@ -657,6 +657,30 @@ int kda_lora_grad(int64_t M, int32_t J, int32_t R, int32_t n, const int32_t* ids
                   hipStream_t stream);
 
 /*
+ * The projection with adapters and its backward, each one call of the products above on one
+ * stream.  how: KDA_LORA_ROWS (forward, as kda_lora_linear_rows), KDA_LORA_WHOLE (kda_lora_linear), or
+ * KDA_LORA_PART, which leaves the adapters' part alone in y or dx for the caller to add the shared
+ * product to (weight is then not read).  x rows have stride ldx, grad_output [M, N] rows ldg.
+ *   forward   u [3, M, R] and y [M, N]
+ *   backward  t [3, M, R] = scale B^T dy (scratch of the caller's, also for da alone), and of dx
+ *             [M, K] bf16, da [n, R, K] and db [n, N, R] f32 those that are not NULL (dx, da need t; db
+ *             needs the forward's u)
+ */
+#define KDA_LORA_ROWS 0
+#define KDA_LORA_WHOLE 1
+#define KDA_LORA_PART 2
+int kda_lora_forward(int64_t M, int32_t N, int32_t K, int32_t R, int32_t n, const int32_t* ids,
+                     int64_t rows_per_id, const void* x, int64_t ldx, const void* weight, const void* lora_a,
+                     const void* lora_b, const float* scale, int32_t how, void* u, void* y,
+                     hipStream_t stream);
+size_t kda_lora_backward_scratch_bytes(int64_t M, int32_t N, int32_t K, int32_t R, int32_t n);
+int kda_lora_backward(int64_t M, int32_t N, int32_t K, int32_t R, int32_t n, const int32_t* ids,
+                      int64_t rows_per_id, const void* x, int64_t ldx, const void* grad_output, int64_t ldg,
+                      const void* weight, const void* lora_a, const void* lora_b, const float* scale,
+                      const void* u, int32_t how, void* t, void* dx, float* da, float* db, void* scratch,
+                      hipStream_t stream);
+
+/*
  * Measurement only (no counterpart in the reference): launches `workgroups` workgroups of
  * four waves; each wave runs `iters` rounds of 8 x 16,384 FLOP of bf16 MFMAs in independent
  * chains with no memory traffic (shape 0: v_mfma_f32_16x16x32_bf16, 8 chains; shape 1:

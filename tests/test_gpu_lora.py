@@ -151,7 +151,7 @@ def test_gpu_refusals():
         with pytest.raises(RuntimeError, match=words):
             lora_linear(e["x"], e["w"], e["a"], e["b"], cuda, e["scale"])
     with pytest.raises(RuntimeError, match="same number of rows"):
-        ops.lora_shrink(d["x"].view(6, 64), d["a"], torch.zeros(4, dtype=torch.int32, device="cuda"), d["scale"])
+        ops.lora_forward(d["x"].view(6, 64), d["w"], d["a"], d["b"], torch.zeros(4, dtype=torch.int32, device="cuda"), d["scale"])
 
 
 def step(d, ids):

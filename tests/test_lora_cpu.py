@@ -114,7 +114,7 @@ def test_refusals():
     refused("adapter_ids", ids=ids.float())
     refused("expected", x=d["x"][0, 0])
     with pytest.raises(RuntimeError, match="ROCm device"):
-        ops.lora_shrink(d["x"][0].bfloat16(), d["a"].bfloat16(), ids, d["scale"])
+        ops.lora_forward(*(d[k].bfloat16() for k in ("x", "w", "a", "b")), ids, d["scale"])
 
 
 @pytest.mark.skipif(not _lib.is_built(), reason="library not built")
@@ -138,5 +138,14 @@ def test_c_abi_refuses_bad_calls_without_gpu():
     refused(expand(4, 16, 8, 2, p, 1, p, p, 0, p, 8, None), "rows of y")
     refused(grad(4, 16, 8, 2, p, 1, p, 16, None, 0, p, p, None), "null")
     refused(grad(4, 16, 8, 2, p, 1, p, 16, p, 0, None, p, None), "null")
+    rows, linear, forward, backward = (getattr(lib, f"kda_lora_{k}") for k in ("linear_rows", "linear", "forward", "backward"))
+    refused(rows(65, 16, 32, 8, 2, p, 1, p, 32, p, p, p, p, p, p, None), "at most 64 rows")
+    refused(rows(4, 16, 24, 8, 2, p, 1, p, 24, p, p, p, p, p, p, None), "in_dim of 32")
+    refused(linear(4, 12, 16, 8, 2, p, 1, p, 16, p, 0, p, p, p, None), "multiples of 8")
+    refused(linear(4, 16, 16, 8, 2, p, 1, p, 16, p, 0, None, p, p, None), "null")
+    refused(forward(4, 16, 32, 8, 2, p, 1, p, 32, p, p, p, p, 3, p, p, None), "unknown way")
+    refused(forward(65, 16, 32, 8, 2, p, 1, p, 32, p, p, p, p, 0, p, p, None), "at most 64 rows")
+    refused(backward(4, 16, 32, 8, 2, p, 1, p, 32, p, 16, p, p, p, p, p, 0, p, p, p, p, p, None), "unknown way")
+    refused(backward(4, 16, 32, 8, 2, p, 1, p, 32, p, 16, p, p, p, p, p, 1, None, p, p, p, p, None), "null")
     assert lib.kda_lora_grad_scratch_bytes(32, 128, 16, 4) == 0  # one range is the result itself
     assert lib.kda_lora_grad_scratch_bytes(8192, 128, 16, 4) > 0
