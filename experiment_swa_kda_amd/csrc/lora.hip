@@ -427,42 +427,39 @@ __global__ __launch_bounds__(256) void lora_grad_kernel(LoraRows rows, int J, in
 
 // The flagged partials of every element, in order: a workgroup lists them, its four waves take every
 // fourth one, eight loads in flight, and their sums meet in LDS.
-constexpr int kGradList = 1024;
+constexpr int kGradSplits = 512;
 __global__ __launch_bounds__(256) void lora_grad_reduce_kernel(int splits, int n, long per,
                                                                const float* __restrict__ part,
                                                                const int32_t* __restrict__ flag,
                                                                float* __restrict__ out) {
-  __shared__ int list[kGradList], s_count;
+  __shared__ int list[kGradSplits], s_count;
   __shared__ f32x4 red[4][kWave];
   const int a = blockIdx.y, g = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const long i = ((long)blockIdx.x * kWave + lane) * 4, ic = i < per ? i : 0;
+  if (g == 0) {
+    int count = 0;
+    for (int s0 = 0; s0 < splits; s0 += kWave) {
+      const int s = s0 + lane;
+      const bool on = s < splits && flag[s * n + a];
+      const unsigned long long m = __ballot(on);
+      if (on) list[count + __popcll(m & ((1ull << lane) - 1))] = s;
+      count += __popcll(m);
+    }
+    if (lane == 0) s_count = count;
+  }
+  __syncthreads();
+  const int count = s_count;
   f32x4 v = zero4();
-  for (int b = 0; b < splits; b += kGradList) {
-    __syncthreads();
-    if (g == 0) {
-      int count = 0;
-      for (int s0 = b; s0 < min(splits, b + kGradList); s0 += kWave) {
-        const int s = s0 + lane;
-        const bool on = s < splits && flag[s * n + a];
-        const unsigned long long m = __ballot(on);
-        if (on) list[count + __popcll(m & ((1ull << lane) - 1))] = s;
-        count += __popcll(m);
-      }
-      if (lane == 0) s_count = count;
-    }
-    __syncthreads();
-    const int count = s_count;
-    for (int k0 = g; k0 < count; k0 += 32) {
-      f32x4 p[8];
+  for (int k0 = g; k0 < count; k0 += 32) {
+    f32x4 p[8];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const int k = k0 + 4 * q;
-        p[q] = *(const f32x4*)(part + ((size_t)list[k < count ? k : g] * n + a) * per + ic);
-        if (k >= count) p[q] = zero4();
-      }
-#pragma unroll
-      for (int q = 0; q < 8; ++q) v += p[q];
+    for (int q = 0; q < 8; ++q) {
+      const int k = k0 + 4 * q;
+      p[q] = *(const f32x4*)(part + ((size_t)list[k < count ? k : g] * n + a) * per + ic);
+      if (k >= count) p[q] = zero4();
     }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v += p[q];
   }
   red[g][lane] = v;
   __syncthreads();
@@ -477,7 +474,7 @@ struct GradPlan {
 // at most 512 MB.
 static GradPlan grad_plan(int64_t M, int32_t J, int32_t R, int32_t n) {
   const int64_t cols = (J + kGradCols - 1) / kGradCols;
-  int64_t splits = (512 + cols - 1) / cols;
+  int64_t splits = (kGradSplits + cols - 1) / cols;
   const int64_t most = ((int64_t)512 << 20) / ((int64_t)n * R * J * 4);
   if (splits > most) splits = most;
   if (splits < 1) splits = 1;

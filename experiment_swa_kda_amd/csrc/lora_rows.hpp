@@ -45,7 +45,7 @@ __device__ __forceinline__ bf16x8 buffer8(__amdgpu_buffer_rsrc_t rs, int off, in
 // is rounded to bf16 (16 bits of u), three where it stays f32.
 __device__ __forceinline__ void split3(float v, bf16& a, bf16& b, bf16& c) {
   a = to_bf16(v);
-  v -= (float)a;
+  v = __builtin_isinf((float)a) ? 0.f : v - (float)a;  // (an infinity is whole in its first part)
   b = to_bf16(v);
   v -= (float)b;
   c = to_bf16(v);

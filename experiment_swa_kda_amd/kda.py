@@ -242,7 +242,7 @@ class _LoraLinear(torch.autograd.Function):
 
 def _cast16(*tensors):
     """bf16 values of the tensors; f32 masters that lie as one launch takes them cast in one."""
-    if all(t.dtype == torch.float32 and t.is_contiguous() and t.numel() % 8 == 0 and t.numel() and t.data_ptr() % 16 == 0
+    if all(t.is_cuda and t.dtype == torch.float32 and t.is_contiguous() and t.numel() % 8 == 0 and t.numel() and t.data_ptr() % 16 == 0
            and t.device == tensors[0].device for t in tensors):
         counts = [t.numel() for t in tensors]
         parts = torch.split(ops.cast_weights_bf16([t.detach() for t in tensors], counts), counts)
@@ -270,6 +270,8 @@ def _check_lora(x, weight, a, b, ids, scaling):
         raise ValueError("lora_linear: lora_a [n, R, K] and lora_b [n, N, R] expected")
     if scaling.shape != a.shape[:1]:
         raise ValueError(f"lora_linear: scaling must have shape {tuple(a.shape[:1])}")
+    if scaling.requires_grad and torch.is_grad_enabled():
+        raise ValueError("lora_linear: scaling is a constant and takes no gradient")
     if ids.dtype not in (torch.int32, torch.int64) or ids.shape not in (x.shape[:1], x.shape[:-1]):
         raise ValueError("lora_linear: adapter_ids int32, one for each sequence (x.shape[:1]) or row (x.shape[:-1])")
     return ids if ids.dtype == torch.int32 else ids.clamp(-1, a.shape[0]).to(torch.int32)
@@ -313,6 +315,8 @@ class LoraLinear(Linear):
 
     def __init__(self, in_features: int, out_features: int, adapters: int, rank: int, alpha: float | None = None):
         super().__init__(in_features, out_features, bias=False)
+        if adapters < 1 or rank < 1:
+            raise ValueError("LoraLinear: at least one adapter of rank 1 expected")
         self.lora_a = nn.Parameter(torch.empty(adapters, rank, in_features))
         self.lora_b = nn.Parameter(torch.zeros(adapters, out_features, rank))
         nn.init.uniform_(self.lora_a, -in_features ** -0.5, in_features ** -0.5)
@@ -326,12 +330,29 @@ class LoraLinear(Linear):
             return lora_linear(x, self.weight, self.lora_a, self.lora_b, self.adapter_ids, self.scaling)
         ids = _check_lora(x, self.weight, self.lora_a, self.lora_b, self.adapter_ids, self.scaling)
         w16 = getattr(self, "_w16", None) if w16 is None else w16
-        a16, b16 = getattr(self, "_lora16", None) or self.adapters_bf16()
+        a16, b16 = self._adapters16()
         return _lora_linear(x, self.weight, self.lora_a, self.lora_b, ids, self.scaling,
                             self.weight.detach().to(torch.bfloat16) if w16 is None else w16, a16, b16)
 
-    def adapters_bf16(self):
-        return tuple(_cast16(self.lora_a, self.lora_b))
+    def keep_adapters_bf16(self):
+        """Keeps bf16 copies of the adapters, used until drop_adapters_bf16 or until one of the masters is
+        replaced or written (as autograd counts writes), so that another request's adapter can be put
+        in a slot.  Returns the copies."""
+        self._lora16 = _cast16(self.lora_a, self.lora_b)
+        masters = (self.lora_a, self.lora_b)
+        self._lora16_of = None if any(p.is_inference() for p in masters) else [
+            (p, p._version, p.detach()) for p in masters]  # (the alias keeps its memory: no other tensor has its address)
+        return self._lora16
+
+    def drop_adapters_bf16(self):
+        self._lora16 = self._lora16_of = None
+
+    def _adapters16(self):
+        if getattr(self, "_lora16", None) is not None and self._lora16_of is not None and all(
+                p is of and p._version == version and p.data_ptr() == alias.data_ptr()
+                for p, (of, version, alias) in zip((self.lora_a, self.lora_b), self._lora16_of)):
+            return self._lora16
+        return _cast16(self.lora_a, self.lora_b)
 
 
 def _norm_gate_eager(x, gate, weight, eps):

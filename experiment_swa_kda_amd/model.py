@@ -732,8 +732,7 @@ class GPT(nn.Module):
                     m._w16 = m.weight.to(torch.bfloat16)
                     out.append(m._w16)
                 if isinstance(m, LoraLinear):
-                    m._lora16 = m.adapters_bf16()
-                    out += m._lora16
+                    out += m.keep_adapters_bf16()
         return out
 
     def drop_bf16_weights(self) -> None:
@@ -745,7 +744,7 @@ class GPT(nn.Module):
             if isinstance(m, Linear):
                 m._w16 = None
             if isinstance(m, LoraLinear):
-                m._lora16 = None
+                m.drop_adapters_bf16()
 
     def add_adapters(self, adapters: int, rank: int, alpha: float | None = None) -> list:
         """Gives the projections behind the mixers (``o_proj``), those of the MLPs and the head a bank of
@@ -753,11 +752,13 @@ class GPT(nn.Module):
         and keep theirs alone).  Returns the new parameters: train these, the rest frozen, with
         ``use_adapters`` naming the adapter of every sequence."""
         new = []
-        for owner, name in [(b.attn, "o_proj") for b in self.transformer.h] + [
-                (b.mlp, name) for b in self.transformer.h for name in ("c_fc", "c_proj")] + [(self, "lm_head")]:
-            old = getattr(owner, name)
-            if type(old) is not Linear:
+        places = [(b.attn, "o_proj") for b in self.transformer.h] + [
+            (b.mlp, name) for b in self.transformer.h for name in ("c_fc", "c_proj")] + [(self, "lm_head")]
+        for owner, name in places:
+            if type(getattr(owner, name)) is not Linear:
                 raise ValueError(f"add_adapters: {name} is no plain Linear (adapters are added once)")
+        for owner, name in places:
+            old = getattr(owner, name)
             m = LoraLinear(old.in_features, old.out_features, adapters, rank, alpha).to(old.weight.device)
             m.weight = old.weight
             setattr(owner, name, m)
@@ -768,9 +769,11 @@ class GPT(nn.Module):
         """The adapter of every sequence of the calls that follow: int32 [B] on the model's device, -1 for
         none; None runs the shared weights alone.  The tensor is read by each call, so a captured call
         follows what is copied into it."""
-        for m in self.modules():
-            if isinstance(m, LoraLinear):
-                m.adapter_ids = adapter_ids
+        banks = [m for m in self.modules() if isinstance(m, LoraLinear)]
+        if not banks and adapter_ids is not None:
+            raise ValueError("use_adapters: the model has no adapters (add_adapters)")
+        for m in banks:
+            m.adapter_ids = adapter_ids
 
     @torch.no_grad()
     def init_weights(self, generator=None):

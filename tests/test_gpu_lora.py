@@ -20,7 +20,7 @@ pytestmark = pytest.mark.gpu
 if torch.cuda.is_available():
     from experiment_swa_kda_amd import KimiDeltaAttention, lora_linear, ops
     from experiment_swa_kda_amd.kda import Linear, LoraLinear
-    from experiment_swa_kda_amd.model import GPT, GPTConfig, KVCache, policy_loss
+    from experiment_swa_kda_amd.model import GPT, GPTConfig, GraphedUpdate, KVCache
 
 
 def n64(t):
@@ -128,6 +128,68 @@ def test_another_requests_nan_and_an_unused_adapters_inf_stay_out(T):
     assert torch.isnan(da[1]).any() and torch.isfinite(y[5]).all()
 
 
+# contraction, outputs and rows of every way a call takes: few rows, rows with ids of their own, whole
+# sequences; one kernel for the projection or the adapters' part beside it, in either direction
+WAYS = [(6, 1, 64, 96), (90, 1, 64, 96), (6, 40, 64, 96), (6, 40, 1608, 72), (6, 40, 72, 1608), (3, 90, 1600, 1544)]
+
+
+@pytest.mark.parametrize("B,T,K,N", WAYS)
+@pytest.mark.parametrize("per_row", [False, True])
+def test_every_way_matches_oracle(B, T, K, N, per_row):
+    d, ids, row_ids = case(B, T, K, N, 24, 3, B + K, masters=True)
+    ids = row_ids if per_row else ids
+    leaves = [d[k].detach().requires_grad_() for k in ("x", "w", "a", "b")]
+    y = lora_linear(*leaves, ids.cuda(), d["scale"])
+    check(d, ids, y, *torch.autograd.grad(y, leaves, d["dy"]))
+
+
+@pytest.mark.parametrize("B,T,K,N", WAYS)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_broken_adapter_in_use_stays_with_its_requests(B, T, K, N, bad):
+    d, _, ids = case(B, T, K, N, 16, 3, 11, masters=True)  # every row its own: tiles of all adapters
+    d["a"][1, 3, 5] = bad
+    d["b"][1, 7] = bad
+    leaves = [d[k].detach().requires_grad_() for k in ("x", "a", "b")]
+    y = lora_linear(leaves[0], d["w"], *leaves[1:], ids.cuda(), d["scale"])
+    dx, da, db = torch.autograd.grad(y, leaves, d["dy"])
+    broken = ids.cuda() == 1
+    assert torch.isfinite(y[~broken]).all() and torch.isfinite(dx[~broken]).all()
+    assert not torch.isfinite(y[broken]).all(-1).any() and not torch.isfinite(dx[broken]).all(-1).any()
+    assert torch.isfinite(da[[0, 2]]).all() and torch.isfinite(db[[0, 2]]).all()
+
+
+@pytest.mark.parametrize("B,T,K,N", WAYS)
+def test_an_infinite_input_is_not_turned_to_nan(B, T, K, N):
+    """x = (inf, 0, ..) and positive weights: every output is the infinity, not infinity - infinity."""
+    d, _, _ = case(B, T, K, N, 8, 2, 12)
+    d["x"].zero_()
+    d["x"][..., 0] = float("inf")
+    for k in ("w", "a", "b"):
+        d[k] = d[k].abs() + 0.5
+    ids = torch.zeros(B, dtype=torch.int32, device="cuda")
+    y = lora_linear(d["x"], d["w"], d["a"], d["b"], ids, d["scale"])
+    assert (y == float("inf")).all()
+
+
+def test_gradient_ranges_of_several_windows():
+    """Long ranges of rows (few ranges for many columns): factor gradients of 5000 rows by 32768 outputs."""
+    g = torch.Generator().manual_seed(13)
+    M, K, N, R, n = 5000, 8, 32768, 8, 3
+    x, dy = (torch.randn(M, k, generator=g).bfloat16().cuda() for k in (K, N))
+    w = torch.zeros(N, K, dtype=torch.bfloat16, device="cuda")
+    a, b = (torch.randn(*s, generator=g).bfloat16().cuda() for s in ((n, R, K), (n, N, R)))
+    scale = torch.ones(n, device="cuda")
+    ids = torch.randint(-1, n, (M,), generator=g).int().cuda()
+    ids[:2100] = 2  # the first steps hold no row of the others
+    _, u = ops.lora_forward(x, w, a, b, ids, scale)
+    _, _, db = ops.lora_backward(x, w, a, b, ids, scale, u, dy, False, False, True)
+    for i in range(n):
+        on = ids == i
+        t = x[on].double() @ a[i].double().t()
+        want, size = dy[on].double().t() @ t, dy[on].double().abs().t() @ (x[on].double().abs() @ a[i].double().abs().t())
+        assert ((db[i] - want).abs() <= (K + M + 64) * 2.0 ** -24 * size).all()
+
+
 def test_empty_and_single():
     d, _, _ = case(2, 3, 64, 96, 16, 2, 8, masters=True)
     for x, ids in ((d["x"][:0], torch.zeros(0)), (d["x"][:, :0], torch.zeros(2))):
@@ -192,6 +254,31 @@ def test_repeats_streams_and_replays_are_bitwise_equal():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(out, both())), k
+
+
+def test_two_captured_calls_take_turns():
+    """Two graphs of the same shapes, replayed by turns and on two streams: neither's workspaces are the other's."""
+    sets = [case(4, 70, 1600, 136, 16, 3, 30 + k, masters=True) for k in range(2)]
+    graphs, outs = [], []
+    ids = [s[1].cuda() for s in sets]
+    want = [step(s[0], i) for s, i in zip(sets, ids)]
+    want = [[t.detach().clone() for t in w] for w in want]
+    for s, i in zip(sets, ids):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(step(s[0], i))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for turn in range(3):
+        for o in outs:
+            for t in o:
+                t.detach().zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert all(torch.equal(p, q) for p, q in zip(o, w)), turn
 
 
 def small_gpt(seed=0):
@@ -281,3 +368,29 @@ def test_decoder_trains_adapters_on_the_policy_loss():
         assert not p[2].any()  # an adapter that no sequence uses
         # both chains round activations and gradients to bf16 (2^-8) at some twenty places
         assert (p - q).norm() <= 0.05 * q.norm()
+
+
+def test_graphed_update_of_adapters_is_the_eager_one():
+    """Three captured updates of the adapters alone leave what three eager ones leave."""
+    def trained(graphed):
+        m = small_gpt(2)
+        for p in m.parameters():
+            p.requires_grad_(False)
+        torch.manual_seed(3)
+        new = m.add_adapters(3, 8)
+        m.use_adapters(torch.tensor([1, -1, 0], dtype=torch.int32, device="cuda"))
+        batch = torch.randint(0, 500, (3, 34), device="cuda")
+        opt = torch.optim.AdamW(new, lr=1e-2, fused=True, capturable=True)
+        update = GraphedUpdate(m, opt, [batch]) if graphed else None
+        for _ in range(3):
+            if graphed:
+                update()
+            else:
+                for p, g in zip(new, torch.autograd.grad(m(batch[:, :-1], batch[:, 1:]), new)):
+                    p.grad = g
+                opt.step()
+        torch.cuda.synchronize()
+        return [p.detach().clone() for p in new]
+
+    for p, q in zip(trained(True), trained(False)):
+        assert torch.equal(p, q)

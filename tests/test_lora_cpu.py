@@ -94,6 +94,35 @@ def test_module_and_decoder_with_adapters():
         gpt.add_adapters(4, 8)
 
 
+def test_adapters_are_added_to_all_projections_or_none():
+    gpt = GPT(GPTConfig(sequence_len=16, vocab_size=50, n_layer=2, n_head=1, n_embd=64, mode="reference"))
+    with pytest.raises(ValueError, match="no adapters"):
+        gpt.use_adapters(torch.tensor([0], dtype=torch.int32))
+    gpt.use_adapters(None)
+    with pytest.raises(ValueError, match="rank"):
+        gpt.add_adapters(2, 0)
+    gpt.transformer.h[1].mlp.c_proj = LoraLinear(256, 64, 1, 8)
+    with pytest.raises(ValueError, match="plain Linear"):
+        gpt.add_adapters(2, 8)
+    assert type(gpt.transformer.h[0].attn.o_proj) is Linear and type(gpt.lm_head) is Linear
+
+
+def test_kept_copies_follow_an_adapter_put_in_a_slot():
+    m = LoraLinear(16, 8, 3, 8)
+    kept = m.keep_adapters_bf16()
+    assert m._adapters16() is kept
+    with torch.no_grad():
+        m.lora_b[1] = 0.5
+    now = m._adapters16()
+    assert now is not kept and torch.equal(now[1], m.lora_b.detach().bfloat16())
+    kept = m.keep_adapters_bf16()
+    assert m._adapters16() is kept
+    m.lora_a = torch.nn.Parameter(torch.ones(3, 8, 16))
+    assert torch.equal(m._adapters16()[0], torch.ones(3, 8, 16).bfloat16())
+    m.drop_adapters_bf16()
+    assert m._lora16 is None
+
+
 def test_refusals():
     d = case(3, 4, 8, 16, 8, 3, dtype=torch.float32)
     ids = torch.zeros(3, dtype=torch.int32)
@@ -113,6 +142,7 @@ def test_refusals():
     refused("adapter_ids", ids=ids[:2])
     refused("adapter_ids", ids=ids.float())
     refused("expected", x=d["x"][0, 0])
+    refused("constant", scale=d["scale"].clone().requires_grad_())
     with pytest.raises(RuntimeError, match="ROCm device"):
         ops.lora_forward(*(d[k].bfloat16() for k in ("x", "w", "a", "b")), ids, d["scale"])
 
