@@ -314,7 +314,8 @@ __global__ __launch_bounds__(kTokThreads) void token_bwd_kernel(
       return;
     }
     const int tc = it.y >= 0 && it.y < vocab ? (int)it.y : -1;
-    const float g = tc < 0 ? __builtin_nanf("") : it.g;  // out-of-range target: its log-probability is NaN
+    // (a target outside the vocabulary has no log-probability, though the row has an entropy)
+    const float g = tc < 0 && it.g != 0.f ? __builtin_nanf("") : it.g;
     const float einv = tok_exp(-it.lse), ge = -g * einv, he = it.h * einv, off = it.ent - it.lse;
     const float2* tabz = tab - (kTabELo << 7);
     auto value = [&](float2 v) {  // the gradient of a column that is not the target

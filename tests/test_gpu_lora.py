@@ -190,6 +190,42 @@ def test_gradient_ranges_of_several_windows():
         assert ((db[i] - want).abs() <= (K + M + 64) * 2.0 ** -24 * size).all()
 
 
+@pytest.mark.parametrize("K,N", [(4096, 64), (64, 4096)])
+@pytest.mark.parametrize("per_row", [False, True])
+def test_offsets_past_32_bits(K, N, per_row):
+    """Inputs or outputs of more than 2^31 elements: the last rows, and the gradients of all."""
+    B, T, R, n = 4, 131500, 8, 3
+    g = torch.Generator().manual_seed(14)
+    small = torch.randn(n, R, K, generator=g) * K ** -0.5, torch.randn(n, N, R, generator=g) * R ** -0.5
+    w = (torch.randn(N, K, generator=g) * K ** -0.5).bfloat16().cuda()
+    torch.manual_seed(14)
+    x, dy = (torch.randn(B, T, k, device="cuda", dtype=torch.bfloat16) for k in (K, N))
+    ids = torch.randint(-1, n, (B, T), generator=g).int() if per_row else torch.tensor([1, -1, 0, 2], dtype=torch.int32)
+    leaves = [x.requires_grad_(), *(v.cuda().requires_grad_() for v in small)]
+    scale = torch.tensor([0.5, 1.0, 1.5]).cuda()
+    y = lora_linear(leaves[0], w, *leaves[1:], ids.cuda(), scale)
+    dx, da, db = torch.autograd.grad(y, leaves, dy)
+    last = slice(T - 96, T)
+    d = dict(x=x[3:, last], dy=dy[3:, last], w=w, a=leaves[1], b=leaves[2], scale=scale)
+    check(d, ids[3:, last] if per_row else ids[3:], y[3:, last], dx[3:, last])
+    want = [[torch.zeros_like(v, dtype=torch.float64) for v in (da, db)] for _ in range(2)]  # and of magnitudes
+    for b in range(B):
+        for t0 in range(0, T, 32875):
+            at = (b, slice(t0, t0 + 32875))
+            row = (ids[at] if per_row else ids[b].expand(T)[at[1]]).cuda()
+            for i in range(n):
+                xi, gi = (v[at][row == i].detach().double() for v in (x, dy))
+                f = [v[i].detach().bfloat16().double() for v in leaves[1:]]
+                for (wa, wb), (X, G, A, F) in zip(want, ((xi, gi, *f), [v.abs() for v in (xi, gi, *f)])):
+                    wa[i] += scale[i].double() * (G @ F).t() @ X
+                    wb[i] += scale[i].double() * G.t() @ (X @ A.t())
+    # a range of at most 32896 rows is a chain of 3 products for each 32 of them, its sum one of some
+    # 32 more; the factor's row (K or N terms) is summed by eight waves or more
+    bound = (3 * 32896 / 32 + 32 + 4096 / 8) * 2.0 ** -24
+    for got, e, size in zip((da, db), *want):
+        assert ((got - e).abs() <= bound * size).all()
+
+
 def test_empty_and_single():
     d, _, _ = case(2, 3, 64, 96, 16, 2, 8, masters=True)
     for x, ids in ((d["x"][:0], torch.zeros(0)), (d["x"][:, :0], torch.zeros(2))):

@@ -319,6 +319,74 @@ def test_losses_together_on_a_side_stream_and_replayed_from_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(out, eager)), k
 
 
+@pytest.mark.parametrize("cols", [1024, 40000])
+def test_two_captured_losses_take_turns(cols):
+    """Two graphs of the same shapes, replayed on two streams: neither's workspaces are the other's."""
+    sets = [[v.cuda() for v in (x, t, old - 6, adv, ref - 6)] for x, t, (old, adv, ref, _) in
+            (case(32, 1000, cols, 40 + k) for k in range(2))]
+    want = [[v.detach().clone() for v in losses(*a, 1000)] for a in sets]
+    graphs, outs = [], []
+    for a in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(losses(*a, 1000))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for turn in range(3):
+        for o in outs:
+            for v in o:
+                v.detach().zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert all(torch.equal(a, b) for a, b in zip(o, w)), turn
+
+
+def test_entropy_gradient_of_a_target_outside_the_vocabulary():
+    """Its log-probability is NaN; the row's entropy and the entropy's gradient are the row's own."""
+    x, t, (_, _, _, h) = case(6, 1000, 1024, 14, ignore_every=0)
+    t[2], t[4] = 1000, -7
+    leaf = x.cuda().requires_grad_()
+    logp, ent = softcap_log_probs(leaf, t.cuda(), 1000, entropy=True)
+    assert torch.isnan(logp).tolist() == [False, False, True, False, True, False]
+    (grad,) = torch.autograd.grad((ent * h.cuda()).sum(), leaf)
+    inside = torch.where((t < 0) | (t >= 1000), 3, t)
+    check_rows(logp[[0, 1, 3, 5]], None, x[[0, 1, 3, 5]], t[[0, 1, 3, 5]], 1000)
+    check_grad(grad, x, inside, 1000, np.zeros(6), n(h))
+
+
+def test_offsets_past_32_bits():
+    """70000 rows of 32768 columns, 2.3e9 logits, with a few counted rows at both ends."""
+    rows, vocab = 70000, 32768
+    x, t, (old, adv, _, _) = case(8, vocab, vocab, 15, ignore_every=0)
+    big = torch.zeros(rows, vocab, dtype=torch.bfloat16, device="cuda")
+    some = torch.tensor([0, 1, 2, 65535, 65536, 69997, 69998, 69999], device="cuda")
+    big[some] = x.cuda()
+    targets = torch.full((rows,), -1, dtype=torch.int64, device="cuda")
+    targets[some] = t.cuda()
+    leaf = big.requires_grad_()
+    logp, ent = softcap_log_probs(leaf, targets, vocab, entropy=True)
+    check_rows(logp[some], ent[some], x, t, vocab)
+    (grad,) = torch.autograd.grad(logp.sum(), leaf)
+    check_grad(grad[some], x, t, vocab, np.ones(8))
+    grad[some] = 0
+    assert not grad.any()
+    del grad
+    full = [torch.zeros(rows, device="cuda").index_put_((some,), v.cuda()) for v in (old - 10, adv)]
+    out = policy_loss(leaf, targets, full[0], full[1], vocab, clip=1.0, clip_high=1e30)
+    assert torch.equal(out.log_probs[some] != 0, torch.ones(8, dtype=torch.bool, device="cuda"))
+    check_rows(out.log_probs[some], None, x, t, vocab)
+    (grad,) = torch.autograd.grad(out.loss, leaf)
+    e_logp = P.rows(n(x), t.tolist(), vocab, CAP)[0]
+    # the slope's error: that of e^(logp - old), EPS and the roundings of logp and the difference
+    slack = 4 * (eps_of(vocab) + 2.0 ** -23 * float(np.abs(e_logp).max() + 16))
+    check_grad(grad[some], x, t, vocab, -np.exp(e_logp - n(old - 10)) * n(adv) / 8, slack=slack)
+    grad[some] = 0
+    assert not grad.any()
+
+
 def test_decoder_trains_on_the_losses():
     """The decoder's own methods: loss values those of its logits, gradients those of the plain
     loss on them, for every parameter."""
