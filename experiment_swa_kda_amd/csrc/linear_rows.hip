@@ -11,7 +11,6 @@
 // 4.7 / 9.1 us of the library GEMM (whose call also takes the host 18 us, this one 8).
 #include "kda_device.hpp"
 #include "kda_host.hpp"
-#include "lora_rows.hpp"
 
 namespace kda {
 
@@ -19,23 +18,12 @@ constexpr int kLinAhead = 3;  // 32-deep steps in flight per wave
 
 enum LinEpilogue { kLinNone = 0, kLinRelu2 = 1, kLinAdd = 2 };
 
-// Low-rank adapters of the rows (LORA): y_m += B_a u_m with a = the row's adapter, u [3, M, R] (three
-// bf16 parts) and factor B [n, N, R].  Rows of different adapters share no product, so the lanes form it with f32
-// FMAs: wave v takes ranks 8 v .. 8 v + 7 (and on, WAVES groups further) of all rows and adds them
-// to its partial tile; the first group's loads are issued ahead of the main loop's.
-struct LinLora {
-  const bf16* u;
-  const bf16* b;
-  LoraRows rows;
-  int R;
-};
-
-template <int MT, int WAVES, bool LORA>
+template <int MT, int WAVES>
 __global__ __launch_bounds__(WAVES * kWave) void linear_rows_kernel(int M, int N, int K, long ldx, int epilogue,
                                                                     const bf16* __restrict__ x,
                                                                     const bf16* __restrict__ w,
                                                                     const bf16* __restrict__ res, long ldr,
-                                                                    bf16* __restrict__ y, LinLora lora) {
+                                                                    bf16* __restrict__ y) {
   __shared__ f32x4 part[WAVES][MT][kWave];
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, lr = lane % 16, kg = lane / 16;
   const int n0 = 16 * blockIdx.x;
@@ -46,34 +34,6 @@ __global__ __launch_bounds__(WAVES * kWave) void linear_rows_kernel(int M, int N
   f32x4 acc[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t) acc[t] = zero4();
-  bf16x8 fb[LORA ? MT : 1][4];
-  bf16x8 fu[LORA ? MT : 1][3];
-  auto load_adapter = [&](int r0) {
-#pragma unroll
-    for (int t = 0; t < (LORA ? MT : 0); ++t) {
-      const int m = 16 * t + lr, a = lora.rows.id(m);
-      const bool ok = a >= 0 && r0 < lora.R;
-#pragma unroll
-      for (int k = 0; k < 3; ++k)
-        fu[t][k] = keep8(*(const bf16x8*)(lora.u + (ok ? ((size_t)k * M + m) * lora.R + r0 : (size_t)0)), ok);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int n = min(n0 + 4 * kg + i, N - 1);
-        fb[t][i] = keep8(*(const bf16x8*)(lora.b + (ok ? ((size_t)a * N + n) * lora.R + r0 : (size_t)0)), ok);
-      }
-    }
-  };
-  auto add_adapter = [&]() {
-#pragma unroll
-    for (int t = 0; t < (LORA ? MT : 0); ++t)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float v = (float)fu[t][0][e] + (float)fu[t][1][e] + (float)fu[t][2][e];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(v, (float)fb[t][i][e], acc[t][i]);
-      }
-  };
-  if constexpr (LORA) load_adapter(8 * wave);
   const int steps = K / 32;  // step s: columns 32 s ..; wave v takes s = v, v + WAVES, ...
   for (int s0 = wave; s0 < steps; s0 += kLinAhead * WAVES) {
     bf16x8 fw[kLinAhead], fx[kLinAhead][MT];
@@ -89,13 +49,6 @@ __global__ __launch_bounds__(WAVES * kWave) void linear_rows_kernel(int M, int N
       if (s0 + u * WAVES < steps)
 #pragma unroll
         for (int t = 0; t < MT; ++t) acc[t] = mfma16(fw[u], fx[u][t], acc[t]);
-  }
-  if constexpr (LORA) {
-    add_adapter();
-    for (int r0 = 8 * (wave + WAVES); r0 < lora.R; r0 += 8 * WAVES) {
-      load_adapter(r0);
-      add_adapter();
-    }
   }
 #pragma unroll
   for (int t = 0; t < MT; ++t) part[wave][t][lane] = acc[t];
@@ -264,51 +217,16 @@ extern "C" int kda_linear_rows(int32_t rows, int32_t out_dim, int32_t in_dim, co
   auto go = [&](auto kern, int waves) {
     hipLaunchKernelGGL(kern, grid, dim3(waves * kWave), 0, stream, rows, out_dim, in_dim, (long)x_row_stride, epilogue,
                        (const bf16*)x, (const bf16*)weight, (const bf16*)residual, (long)residual_row_stride,
-                       (bf16*)y, LinLora{});
+                       (bf16*)y);
   };
   // a long contraction over few workgroups: twice the waves
   const bool deep = in_dim >= 1024;
   if (rows <= 16)
-    deep ? go(linear_rows_kernel<1, 8, false>, 8) : go(linear_rows_kernel<1, 4, false>, 4);
+    deep ? go(linear_rows_kernel<1, 8>, 8) : go(linear_rows_kernel<1, 4>, 4);
   else if (rows <= 32)
-    deep ? go(linear_rows_kernel<2, 8, false>, 8) : go(linear_rows_kernel<2, 4, false>, 4);
+    deep ? go(linear_rows_kernel<2, 8>, 8) : go(linear_rows_kernel<2, 4>, 4);
   else
-    deep ? go(linear_rows_kernel<4, 8, false>, 8) : go(linear_rows_kernel<4, 4, false>, 4);
+    deep ? go(linear_rows_kernel<4, 8>, 8) : go(linear_rows_kernel<4, 4>, 4);
   KDA_LAUNCH_CHECK("linear_rows");
-  return KDA_OK;
-}
-
-extern "C" int kda_lora_linear_rows(int32_t rows, int32_t out_dim, int32_t in_dim, int32_t R, int32_t n,
-                                    const int32_t* ids, int64_t rows_per_id, const void* x, int64_t x_row_stride,
-                                    const void* weight, const void* lora_a, const void* lora_b, const float* scale,
-                                    void* u, void* y, hipStream_t stream) {
-  using namespace kda;
-  KDA_REQUIRE(rows >= 0 && rows <= 64, "lora_linear_rows: at most 64 rows");
-  KDA_REQUIRE(out_dim > 0 && out_dim % 4 == 0 && in_dim > 0 && in_dim % 32 == 0,
-              "lora_linear_rows: out_dim must be a multiple of 4, in_dim of 32");
-  int rc = check_lora("lora_linear_rows", rows, in_dim, R, n, ids, rows_per_id);
-  if (rc != KDA_OK) return rc;
-  KDA_REQUIRE(x_row_stride >= in_dim && x_row_stride % 8 == 0, "lora_linear_rows: x rows must be 16-byte aligned");
-  if (rows == 0) return KDA_OK;
-  KDA_REQUIRE(x && weight && lora_a && lora_b && u && y && aligned16(x, weight, lora_a, lora_b, u, y),
-              "lora_linear_rows: null or unaligned pointer");
-  const LoraRows lr{rows, n, ids, (int)rows_per_id};
-  hipLaunchKernelGGL(lora_shrink_rows_kernel<4>, dim3((unsigned)rows, (unsigned)((R + 3) / 4)), dim3(256), 0, stream, lr,
-                     in_dim, R, (const bf16*)x, (long)x_row_stride, (const bf16*)lora_a, scale, (bf16*)u);
-  KDA_LAUNCH_CHECK("lora_shrink_rows");
-  const dim3 grid((unsigned)((out_dim + 15) / 16));
-  auto go = [&](auto kern, int waves) {
-    hipLaunchKernelGGL(kern, grid, dim3(waves * kWave), 0, stream, rows, out_dim, in_dim, (long)x_row_stride, kLinNone,
-                       (const bf16*)x, (const bf16*)weight, (const bf16*)nullptr, 0L, (bf16*)y,
-                       LinLora{(const bf16*)u, (const bf16*)lora_b, lr, R});
-  };
-  const bool deep = in_dim >= 1024;
-  if (rows <= 16)
-    deep ? go(linear_rows_kernel<1, 8, true>, 8) : go(linear_rows_kernel<1, 4, true>, 4);
-  else if (rows <= 32)
-    deep ? go(linear_rows_kernel<2, 8, true>, 8) : go(linear_rows_kernel<2, 4, true>, 4);
-  else
-    deep ? go(linear_rows_kernel<4, 8, true>, 8) : go(linear_rows_kernel<4, 4, true>, 4);
-  KDA_LAUNCH_CHECK("lora_linear_rows");
   return KDA_OK;
 }

@@ -17,10 +17,6 @@
 
 namespace kda {
 
-// A row of 64 bf16 in LDS is 128 bytes; its 16-byte chunk c sits in slot c ^ (row % 8), so that the
-// same chunk of eight neighbouring rows, and all chunks of one, fall on different banks.
-__device__ __forceinline__ int row64_off(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
-
 // ---------------------------------------------------------------------------------------
 // shrink: one workgroup per 16 MT rows; its waves take 64 columns of J at a time each, and their
 // partial tiles meet in LDS.  RT = ceil(R / 16).  Lanes load along rows (8 lanes to a 128-byte line:

@@ -1,4 +1,4 @@
-// The rows of a call with low-rank adapters, and its checks (lora.hip, linear_rows.hip).
+// The rows of a call with low-rank adapters, and its checks (lora.hip, lora_linear.hip, lora_linear_rows.hip).
 #pragma once
 
 #include "kda_device.hpp"
@@ -39,6 +39,10 @@ __device__ __forceinline__ bf16x8 buffer8(__amdgpu_buffer_rsrc_t rs, int off, in
   const i4 v = __builtin_amdgcn_raw_buffer_load_b128(rs, off, uniform, 0);
   return __builtin_bit_cast(bf16x8, v);
 }
+
+// A row of 64 bf16 in LDS is 128 bytes; its 16-byte chunk c sits in slot c ^ (row % 8), so that the
+// same chunk of eight neighbouring rows, and all chunks of one, fall on different banks.
+__device__ __forceinline__ int row64_off(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
 
 // u [3, M, R]: an f32 value as the sum of three bf16 parts, each the rounding of what the ones before
 // leave (24 bits together), so that the matrix cores take it as it lies: two parts where the result

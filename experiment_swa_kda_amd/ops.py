@@ -808,6 +808,9 @@ def embedding_backward(idx, grad_output, vocab):
     return dw
 
 
+_LORA_ROWS = 64  # the most rows kda_lora_linear_rows takes
+
+
 def _lora_way(M, K, N):
     """How a contraction of K with its adapters runs best on M rows and N outputs: as one kernel, or the
     adapters' part alone with a library product added to it.  One kernel takes 22 us against 43 for M 8192,
@@ -843,7 +846,7 @@ def lora_forward(x, w16, a, b, ids, scale):
     (M, K), N, (n, R) = x.shape, w16.shape[0], a.shape[:2]
     u = torch.empty(3, M, R, dtype=torch.bfloat16, device=dev)
     y = torch.empty(M, N, dtype=torch.bfloat16, device=dev)
-    how = KDA_LORA_ROWS if M <= _LINEAR_ROWS and K % 32 == 0 else _lora_way(M, K, N)
+    how = KDA_LORA_ROWS if M <= _LORA_ROWS else _lora_way(M, K, N)
     with _on(dev):
         rc = _lib.load().kda_lora_forward(M, N, K, R, n, ptr(ids), per, ptr(x), K, ptr(w16), ptr(a), ptr(b), ptr(scale),
                                           how, ptr(u), ptr(y), _stream(dev))

@@ -635,7 +635,7 @@ int kda_lora_expand(int64_t M, int32_t J, int32_t R, int32_t n, const int32_t* i
                     const void* u, const void* factor, int32_t factor_cols, void* y, int64_t ldy,
                     hipStream_t stream);
 /*
- * The whole of y = x W^T + s B (A x) for at most 64 rows (in_dim a multiple of 32): weight
+ * The whole of y = x W^T + s B (A x) for at most 64 rows (out_dim a multiple of 8): weight
  * [out_dim, in_dim], lora_a [n, R, in_dim], lora_b [n, out_dim, R] bf16, rounded once; u [3, rows,
  * R] receives s A x.
  */
