@@ -21,7 +21,7 @@ namespace kda {
 // shrink: one workgroup per 16 MT rows; its waves take 64 columns of J at a time each, and their
 // partial tiles meet in LDS.  RT = ceil(R / 16).  Lanes load along rows (8 lanes to a 128-byte line:
 // an MFMA fragment loaded directly has 16 rows in 16 neighbouring lanes, 64 cycles of address
-// processing for its 1 KB instead of 16: 7777 x 4096 at rank 64 took 48 us) and pass the rows
+// processing for its 1 KB instead of 16: 7777 x 4096 at rank 64 took 48 us, now 12, 5.2 TB/s) and pass the rows
 // through an LDS stage of their own, so without a barrier; AHEAD groups of 64 columns are in flight.
 // TRANSPOSED: F is [n, J, R], its fragments run down the stage's columns.
 // ---------------------------------------------------------------------------------------
@@ -176,7 +176,8 @@ __global__ __launch_bounds__(kShrinkWaves * kWave) void lora_shrink_kernel(LoraR
 // expand: 64 rows x 256 columns per workgroup; wave w has rows 16 w .. and keeps their u in
 // registers.  KS = ceil(R / 32) steps of the contraction.  F passes through LDS in pieces of 64
 // columns, the next piece on its way; so does the result, to be stored along rows.  TRANSPOSED: F is
-// [n, R, J].
+// [n, R, J].  Bound by the write of y: 7777 x 2048 and x 4096 at rank 64 take 13 and 18 us (2.4 and 3.5
+// TB/s), 8192 x 32768 at rank 16 156 us (3.4).
 // ---------------------------------------------------------------------------------------
 constexpr int kExpandCols = 256;
 
@@ -286,8 +287,11 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraRows rows, int J, 
 
 // Rows that each have an id of their own (a token of every request): tiles would hold as many
 // adapters as rows, so every row takes its own products with vector FMAs (lora_shrink_rows_kernel,
-// and here a thread per column of y, whose R factors lie together).
-constexpr int kLoraRowsMost = 512;
+// and here a thread per column of y, whose R factors lie together).  Rank 16, 384 -> 1536, shrink + expand
+// + the library's product, ids drawn from 8 and from M adapters, against tiles: M 256 12 and 12 us (36
+// and 149), M 1024 23 and 24 (39 and 195); beyond, neighbours mostly share an adapter (M 2048, four runs: 36
+// us against 21).
+constexpr int kLoraRowsMost = 1024;
 __global__ __launch_bounds__(256) void lora_expand_rows_kernel(LoraRows rows, int J, int R, const bf16* __restrict__ u,
                                                                const bf16* __restrict__ f, bf16* __restrict__ y,
                                                                long ldy) {
@@ -313,6 +317,8 @@ __global__ __launch_bounds__(256) void lora_expand_rows_kernel(LoraRows rows, in
 // that hold a row of the adapter, with the other rows masked and the next step's loads in flight, and
 // leaves an f32 partial and a flag; a second kernel sums the flagged partials in order.  A single
 // range is the result itself (flag null).  COLS: the result is [n, J, R], else [n, R, J].
+// Bound by reading x once and u once for every 128 columns: 8192 x 32768 at rank 16 takes 122 us with
+// the sum (4.4 TB/s), 7777 x 4096 at rank 64, three adapters, 36 + 6 (the ranges' partials are 18 MB).
 // ---------------------------------------------------------------------------------------
 constexpr int kGradCols = 128;
 constexpr int kGradRows = 64;
@@ -468,6 +474,9 @@ struct GradPlan {
 
 // Ranges of rows: enough (column block, range) workgroups to fill the chip twice, and partials of
 // at most 512 MB.
+// Ranges for 512 workgroups of one adapter; more of them shorten a range but add partials (8192 x 4096 at
+// rank 32: 32 / 27 / 29 / 32 us for 512 / 768 / 1024 / 1536, 7777 x 4096 at rank 64 39 / 41 / 36 / 44,
+// 8192 x 1536 at rank 16 18 / 18 / 21 / 26).  Partials stay under 512 MB.
 static GradPlan grad_plan(int64_t M, int32_t J, int32_t R, int32_t n) {
   const int64_t cols = (J + kGradCols - 1) / kGradCols;
   int64_t splits = (kGradSplits + cols - 1) / cols;
@@ -506,8 +515,9 @@ extern "C" int kda_lora_shrink(int64_t M, int32_t J, int32_t R, int32_t n, const
     hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(kShrinkWaves * kWave), 0, stream, rows, seq_tiles, J, R,
                        (const bf16*)x, (long)ldx, (const bf16*)factor, scale, (bf16*)u);
   };
-  // 32 rows share a read of the factor where that still leaves work for every CU
-  auto pick = [&](auto k1, auto k2) { M >= 4096 ? go(k2, 2) : go(k1, 1); };
+  // 32 rows share a read of the factor where that leaves work for every CU: 65536 x 4096 at rank 128 takes
+  // 225 us against 332 in tiles of 16, 8192 x 1536 at rank 16 5.7 / 6.3, but 4096 x 4096 at rank 64 16.3 / 13.0
+  auto pick = [&](auto k1, auto k2) { M >= 8192 ? go(k2, 2) : go(k1, 1); };
   if (factor_cols) {
     if (R <= 16) pick(lora_shrink_kernel<1, 1, true>, lora_shrink_kernel<1, 2, true>);
     else if (R <= 32) pick(lora_shrink_kernel<2, 1, true>, lora_shrink_kernel<2, 2, true>);

@@ -809,14 +809,15 @@ def embedding_backward(idx, grad_output, vocab):
 
 
 _LORA_ROWS = 64  # the most rows kda_lora_linear_rows takes
+_LORA_ROW_IDS = 1024  # the most rows of own ids that the adapters' kernels take one by one
 
 
 def _lora_way(M, K, N):
     """How a contraction of K with its adapters runs best on M rows and N outputs: as one kernel, or the
     adapters' part alone with a library product added to it.  One kernel takes 22 us against 43 for M 8192,
-    K 384, N 1536, 20 / 28 for 8192 x 768 x 768, 9 / 18 for 2048 x 384 x 1536, 22 / 27 for 8192 x 1536 x 384,
-    but 20 / 17 for 2048 x 1536 x 384 (48 tiles), 105 / 84 for 8192 x 1024 x 4096 and 165 / 111 for 7777 x
-    4096 x 2048 (the library's larger tiles)."""
+    K 384, N 1536, 21 / 28 for 8192 x 768 x 768, 12 / 21 for 2048 x 384 x 1536, 21 / 27 for 8192 x 1536 x 384,
+    but 20 / 17 for 2048 x 1536 x 384 (48 tiles), 79 / 71 for the transposed 8192 x 4096 x 1024 and 163 / 111
+    for 7777 x 4096 x 2048 (the library's larger tiles read their operands half as often)."""
     whole = K <= 768 or (K <= 1536 and N <= 1024 and -(-M // 128) * -(-N // 128) >= 128)
     return KDA_LORA_WHOLE if whole else KDA_LORA_PART
 
@@ -846,7 +847,12 @@ def lora_forward(x, w16, a, b, ids, scale):
     (M, K), N, (n, R) = x.shape, w16.shape[0], a.shape[:2]
     u = torch.empty(3, M, R, dtype=torch.bfloat16, device=dev)
     y = torch.empty(M, N, dtype=torch.bfloat16, device=dev)
-    how = KDA_LORA_ROWS if M <= _LORA_ROWS else _lora_way(M, K, N)
+    if M <= _LORA_ROWS:
+        how = KDA_LORA_ROWS
+    elif per == 1 and M <= _LORA_ROW_IDS:
+        how = KDA_LORA_PART  # (one kernel's tiles of as many adapters as rows: M 256, K 384, N 1536 85 us, this 12)
+    else:
+        how = _lora_way(M, K, N)
     with _on(dev):
         rc = _lib.load().kda_lora_forward(M, N, K, R, n, ptr(ids), per, ptr(x), K, ptr(w16), ptr(a), ptr(b), ptr(scale),
                                           how, ptr(u), ptr(y), _stream(dev))
