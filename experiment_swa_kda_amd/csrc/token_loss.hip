@@ -145,6 +145,8 @@ struct TokOut {
 // Forward of many rows: one wave per row, so that a row's sums are a wave's and no barrier stalls
 // the loads; the next chunk's loads, also the next row's, are in flight while one is summed.  Rows
 // go last to first: the ones the projection before wrote last are still in the memory-side cache.
+// Bound by that read: 8192 x 32768 takes 99 us, 5.4 TB/s, with the entropy 3001 x 50000 90 us, 3.3 (two
+// table values an element).
 template <bool ENT>
 __global__ __launch_bounds__(kTokThreads) void token_fwd_kernel(long rows, int vocab, long stride, float cap,
                                                                 const bf16* __restrict__ logits,
@@ -271,6 +273,8 @@ __global__ __launch_bounds__(kTokWide) void token_fwd_wide_kernel(long rows, int
 
 // Backward for given row gradients: g of logp (times *scale if given) and, with ENT, h of the
 // entropy.  Nothing is reduced, so (row, chunk) items go to the waves in order.
+// Bound by one read and one write: 8192 x 32768 takes 179 us behind the forward (last-level cache) and 204
+// alone, 5.3 TB/s; with the entropy 3001 x 50000 107 us, 5.6.
 template <bool ENT>
 __global__ __launch_bounds__(kTokThreads) void token_bwd_kernel(
     long rows, int vocab, long stride, float cap, const bf16* __restrict__ logits, const int64_t* __restrict__ targets,
@@ -423,6 +427,8 @@ __device__ __forceinline__ double wave_sum64(double v) {
 // LDS), log-probabilities and loss terms after them; in between every thread only adds the
 // partials and forms the slope from two hardware exponentials.  part[workgroup] = f64 sums of its
 // rows' (loss, KL, clipped weight), for policy_sum_kernel.
+// Bound by one read and one write: 8192 x 32768 takes 198 us, 5.4 TB/s (the two passes 303; with workgroups
+// of 512 threads and eight vectors each 266), 500 x 8003 15 us.
 constexpr int kFusedMaxVec = 4;
 constexpr int kFusedMost = 1024;                       // threads of the widest workgroup
 constexpr int kFusedMaxCols = kFusedMost * 8 * kFusedMaxVec;
@@ -735,6 +741,7 @@ __global__ __launch_bounds__(kRowsThreads) void policy_rows_kernel(long rows, co
 // partner of i.  Sequence s holds rows T s .. T s + T - 1, or cu[s] .. cu[s + 1] - 1.  One workgroup;
 // a wave sums a sequence, in 64 bits and a fixed order.  Sequence bounds that are no
 // non-decreasing walk inside the rows make every output NaN (nothing is read outside the rows).
+// Bound by the latency of its few dependent steps: 5.4 us for 4 pairs of 764 rows in all, 6.7 for 8192.
 // ---------------------------------------------------------------------------------------
 constexpr int kPairAhead = 8;
 __global__ __launch_bounds__(kRowsThreads) void preference_pairs_kernel(
