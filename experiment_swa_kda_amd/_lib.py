@@ -111,7 +111,7 @@ SIGNATURES = {
     "kda_lora_linear": (ctypes.c_int, [_L, _I, _I, _I, _I, _P, _L, _P, _L, _P, _I, _P, _P, _P, _P]),
     "kda_lora_forward": (ctypes.c_int, [_L, _I, _I, _I, _I, _P, _L, _P, _L, _P, _P, _P, _P, _I, _P, _P, _P]),
     "kda_lora_backward_scratch_bytes": (ctypes.c_size_t, [_L, _I, _I, _I, _I]),
-    "kda_lora_backward": (ctypes.c_int, [_L, _I, _I, _I, _I, _P, _L, _P, _L, _P, _L] + [_P] * 5 + [_I] + [_P] * 6),
+    "kda_lora_backward": (ctypes.c_int, [_L, _I, _I, _I, _I, _P, _L, _P, _L, _P, _L] + [_P] * 5 + [_I] + [_P] * 5),
     "kda_lora_shrink": (ctypes.c_int, [_L, _I, _I, _I, _P, _L, _P, _L, _P, _I, _P, _P, _P]),
     "kda_lora_expand": (ctypes.c_int, [_L, _I, _I, _I, _P, _L, _P, _P, _I, _P, _L, _P]),
     "kda_lora_grad_scratch_bytes": (ctypes.c_size_t, [_L, _I, _I, _I]),

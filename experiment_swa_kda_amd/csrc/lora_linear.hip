@@ -268,24 +268,30 @@ extern "C" int kda_lora_forward(int64_t M, int32_t N, int32_t K, int32_t R, int3
   return kda_lora_expand(M, N, R, n, ids, rows_per_id, u, lora_b, 1, y, N, stream);
 }
 
+// t = s B^T dy in its three parts, then the factor gradients' partials (one gradient after the other)
+static size_t lora_t_bytes(int64_t M, int32_t R) { return M > 0 && R > 0 ? kda::align256((size_t)3 * M * R * 2) : 0; }
+
 extern "C" size_t kda_lora_backward_scratch_bytes(int64_t M, int32_t N, int32_t K, int32_t R, int32_t n) {
   const size_t a = kda_lora_grad_scratch_bytes(M, K, R, n), b = kda_lora_grad_scratch_bytes(M, N, R, n);
-  return a > b ? a : b;
+  return lora_t_bytes(M, R) + (a > b ? a : b);
 }
 
 extern "C" int kda_lora_backward(int64_t M, int32_t N, int32_t K, int32_t R, int32_t n, const int32_t* ids,
                                  int64_t rows_per_id, const void* x, int64_t ldx, const void* grad_output, int64_t ldg,
                                  const void* weight, const void* lora_a, const void* lora_b, const float* scale,
-                                 const void* u, int32_t how, void* t, void* dx, float* da, float* db, void* scratch,
+                                 const void* u, int32_t how, void* dx, float* da, float* db, void* scratch,
                                  hipStream_t stream) {
   KDA_REQUIRE(how == KDA_LORA_WHOLE || how == KDA_LORA_PART, "lora_backward: unknown way");
+  KDA_REQUIRE(M <= 0 || scratch, "lora_backward: null scratch");
+  void* t = scratch;
+  void* part = scratch ? (char*)scratch + lora_t_bytes(M, R) : nullptr;
   int rc = KDA_OK;
   if (dx || da) rc = kda_lora_shrink(M, N, R, n, ids, rows_per_id, grad_output, ldg, lora_b, 1, scale, t, stream);
   if (rc == KDA_OK && dx)
     rc = how == KDA_LORA_WHOLE
              ? kda_lora_linear(M, K, N, R, n, ids, rows_per_id, grad_output, ldg, weight, 1, t, lora_a, dx, stream)
              : kda_lora_expand(M, K, R, n, ids, rows_per_id, t, lora_a, 0, dx, K, stream);
-  if (rc == KDA_OK && da) rc = kda_lora_grad(M, K, R, n, ids, rows_per_id, x, ldx, t, 0, da, scratch, stream);
-  if (rc == KDA_OK && db) rc = kda_lora_grad(M, N, R, n, ids, rows_per_id, grad_output, ldg, u, 1, db, scratch, stream);
+  if (rc == KDA_OK && da) rc = kda_lora_grad(M, K, R, n, ids, rows_per_id, x, ldx, t, 0, da, part, stream);
+  if (rc == KDA_OK && db) rc = kda_lora_grad(M, N, R, n, ids, rows_per_id, grad_output, ldg, u, 1, db, part, stream);
   return rc;
 }

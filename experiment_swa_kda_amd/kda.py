@@ -29,6 +29,8 @@ from __future__ import annotations
 
 from dataclasses import dataclass
 
+import functools
+
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
@@ -214,30 +216,42 @@ def linear_few_rows(m, x, *, relu2=False, residual=None):
     return ops.linear_rows(x, w16, relu2=relu2, residual=residual)
 
 
+def once(backward):
+    """``once_differentiable`` without its bookkeeping (5 us of a call) in a pass that is not recorded."""
+    recorded = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def call(ctx, *grads):
+        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return call
+
+
 class _LoraLinear(torch.autograd.Function):
-    """A projection with adapters, for autograd: bf16 W, A and B (casts of the masters, whose gradients
-    come back in f32)."""
+    """A projection with adapters, for autograd: contiguous rows x2 and bf16 W, A and B (casts of the
+    masters, whose gradients come back in f32), checked; ids for ``per`` rows each."""
 
     @staticmethod
-    def forward(ctx, x, weight, a, b, ids, scaling, w16, a16, b16):
-        x2 = x.reshape(-1, x.shape[-1])
-        y, u = ops.lora_forward(x2, w16, a16, b16, ids, scaling)
+    def forward(ctx, x, weight, a, b, per, x2, w16, a16, b16, ids, scaling):
+        dev = x2.device
+        y, u = ops._lora_forward(dev, per, x2, w16, a16, b16, ids, scaling)
         ctx.save_for_backward(x2, w16, a16, b16, ids, scaling, u)
+        ctx.args = dev, per
         ctx.shape, ctx.types = x.shape, (weight.dtype, a.dtype, b.dtype)
         return y.view(*x.shape[:-1], w16.shape[0])
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, grad):
-        x2, w16, a16, b16, ids, scaling, u = ctx.saved_tensors
+        x2, w16, *_ = saved = ctx.saved_tensors
         need = ctx.needs_input_grad
-        g2 = grad.reshape(-1, grad.shape[-1]).to(torch.bfloat16)
-        dx, da, db = ops.lora_backward(x2, w16, a16, b16, ids, scaling, u, g2, need[0], need[2], need[3])
+        g2 = ops._c(grad.reshape(x2.shape[0], w16.shape[0]))
+        dx, da, db = ops._lora_backward(*ctx.args, *saved, g2, need[0], need[2], need[3])
         dw = None
         if need[1]:
             dw = (ops.weight_grad(g2, x2) if w16.numel() <= _SPLIT_WGRAD_MAX else _mm_f32(g2.t(), x2)).to(ctx.types[0])
         return (dx.view(ctx.shape) if need[0] else None, dw, da.to(ctx.types[1]) if need[2] else None,
-                db.to(ctx.types[2]) if need[3] else None, None, None, None, None, None)
+                db.to(ctx.types[2]) if need[3] else None, None, None, None, None, None, None, None)
 
 
 def _cast16(*tensors):
@@ -251,14 +265,19 @@ def _cast16(*tensors):
 
 
 def _lora_linear(x, weight, a, b, ids, scaling, w16, a16, b16):
-    """The projection with adapters on the HIP kernels; outside autograd's and the transforms' sight
-    where nothing is to be recorded."""
+    """The projection with adapters on the HIP kernels, shapes checked; outside autograd's and the
+    transforms' sight where nothing is to be recorded."""
+    dev = ops._require_cuda("lora_linear", x, w16, a16, b16, ids, scaling)
     ids = ids if ids.is_contiguous() else ids.contiguous()
-    scaling = scaling if scaling.dtype == torch.float32 else scaling.detach().float()
-    if not _needs_grad(x, weight, a, b) and _untransformed(x, weight, a, b, ids, scaling):
-        y, _ = ops.lora_forward(x.reshape(-1, x.shape[-1]), w16, a16, b16, ids, scaling)
-        return y.view(*x.shape[:-1], w16.shape[0])
-    return _LoraLinear.apply(x, weight, a, b, ids, scaling, w16, a16, b16)
+    scaling = ops._c(scaling if scaling.dtype == torch.float32 else scaling.detach().float())
+    x2 = x if x.ndim == 2 else x.reshape(-1, x.shape[-1])
+    per = (x2.shape[0] // ids.numel() if ids.numel() else 0) or 1
+    recorded = _needs_grad(x, weight, a, b) or not _untransformed(x, weight, a, b, ids, scaling)
+    args = per, ops._c(x2.detach() if recorded else x2), ops._c(w16), ops._c(a16), ops._c(b16), ids, scaling
+    if recorded:
+        return _LoraLinear.apply(x, weight, a, b, *args)
+    y, _ = ops._lora_forward(dev, *args)
+    return y if x.ndim == 2 else y.view(*x.shape[:-1], w16.shape[0])
 
 
 def _check_lora(x, weight, a, b, ids, scaling):

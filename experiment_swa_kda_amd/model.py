@@ -22,10 +22,9 @@ from typing import NamedTuple
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from . import ops
-from .kda import KDAState, KimiDeltaAttention, Linear, LoraLinear, linear_few_rows, plain
+from .kda import KDAState, KimiDeltaAttention, Linear, LoraLinear, linear_few_rows, once, plain
 
 
 @dataclass
@@ -200,6 +199,7 @@ class _SoftcapLogProbs(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, targets, vocab, softcap, ignore_index, entropy):
+        logits, targets = ops._c(logits), ops._c(targets)
         logp, lse, ent = ops.softcap_log_probs_forward(logits, targets, vocab, softcap, ignore_index, entropy=entropy)
         ctx.save_for_backward(logits, targets, lse, ent)
         ctx.args = (vocab, softcap, ignore_index)
@@ -207,12 +207,13 @@ class _SoftcapLogProbs(torch.autograd.Function):
         return logp, ent
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, g, h):
-        logits, targets, lse, ent = ctx.saved_tensors
         if g is None and h is None:
             return (None,) * 6
-        return (ops.softcap_log_probs_backward(logits, targets, lse, ent, g, h, *ctx.args), *(None,) * 5)
+        logits, targets, lse, ent = ctx.saved_tensors
+        return (ops._softcap_log_probs_backward(logits.device, logits, targets, lse, ent, ops._c(g), ops._c(h), *ctx.args,
+                                                None), *(None,) * 5)
 
 
 class _PolicyLoss(torch.autograd.Function):
@@ -221,19 +222,23 @@ class _PolicyLoss(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, targets, old, adv, ref, weights, vocab, softcap, ignore_index, lo, hi, kl_coef, grad):
+        logits, targets = ops._c(logits), ops._c(targets)
         logp, lse, _ = ops.softcap_log_probs_forward(logits, targets, vocab, softcap, ignore_index)
         loss, stats, slope = ops.policy_rows(targets, logp, old, adv, ref, weights, lo, hi, kl_coef, ignore_index,
                                              slopes=grad)
         ctx.save_for_backward(logits, targets, lse, slope)
         ctx.args = (vocab, softcap, ignore_index)
         ctx.mark_non_differentiable(logp, stats)
+        ctx.set_materialize_grads(False)
         return loss, logp, stats
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, grad, _logp, _stats):
+        if grad is None:
+            return (None,) * 13
         logits, targets, lse, slope = ctx.saved_tensors
-        return (ops.softcap_log_probs_backward(logits, targets, lse, None, slope, None, *ctx.args, scale=grad),
+        return (ops._softcap_log_probs_backward(logits.device, logits, targets, lse, None, slope, None, *ctx.args, grad),
                 *(None,) * 12)
 
 
@@ -251,16 +256,19 @@ class _PolicyLossFused(torch.autograd.Function):
         ctx.expected = expected_grad
         ctx.used = False
         ctx.mark_non_differentiable(logp, stats)
+        ctx.set_materialize_grads(False)
         return loss, logp, stats
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, grad, _logp, _stats):
+        if grad is None:
+            return (None,) * 13
         if ctx.used:  # the gradient buffer is handed out (and rescaled) in place
             raise RuntimeError("policy_loss: the fused form's backward can run only once")
         ctx.used = True
         (dlogits,) = ctx.saved_tensors
-        ops.rescale_bf16_if_changed(dlogits, grad, ctx.expected)
+        ops._rescale_bf16_if_changed(dlogits.device, dlogits, grad, ctx.expected)
         return (dlogits, *(None,) * 12)
 
 
@@ -271,19 +279,23 @@ class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, pairs, seq_len, cu_seqlens, ref, vocab, softcap, ignore_index, beta, smoothing,
                 average, grad):
+        logits, targets = ops._c(logits), ops._c(targets)
         logp, lse, _ = ops.softcap_log_probs_forward(logits, targets, vocab, softcap, ignore_index, double=True)
         loss, seq, margins, slope = ops.preference_pairs(targets, logp, pairs, seq_len, cu_seqlens, ref, beta,
                                                          smoothing, average, ignore_index, slopes=grad)
         ctx.save_for_backward(logits, targets, lse, slope)
         ctx.args = (vocab, softcap, ignore_index)
         ctx.mark_non_differentiable(seq, margins)
+        ctx.set_materialize_grads(False)
         return loss, seq, margins
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, grad, _seq, _margins):
+        if grad is None:
+            return (None,) * 13
         logits, targets, lse, slope = ctx.saved_tensors
-        return (ops.softcap_log_probs_backward(logits, targets, lse, None, slope, None, *ctx.args, scale=grad),
+        return (ops._softcap_log_probs_backward(logits.device, logits, targets, lse, None, slope, None, *ctx.args, grad),
                 *(None,) * 12)
 
 
@@ -294,8 +306,14 @@ def _flat_tokens(what, logits, targets, vocab, *rows):
         raise ValueError(f"{what}: logits [..., columns] and one target and row value for each leading position expected")
     if not 0 < vocab <= logits.shape[-1]:
         raise ValueError(f"{what}: vocab must be in [1, {logits.shape[-1]}]")
-    return (logits.reshape(-1, logits.shape[-1]), targets.reshape(-1),
-            *(None if t is None else t.detach().reshape(-1).float() for t in rows))
+    flat = logits if logits.ndim == 2 else logits.reshape(-1, logits.shape[-1])
+    return (flat, targets if targets.ndim == 1 else targets.reshape(-1), *(None if t is None else _row_values(t) for t in rows))
+
+
+def _row_values(t):
+    t = t.detach() if t.requires_grad else t
+    t = t if t.ndim == 1 else t.reshape(-1)
+    return t if t.dtype == torch.float32 else t.float()
 
 
 def _eager_log_probs(logits, targets, vocab, softcap, ignore_index):
@@ -319,7 +337,9 @@ def softcap_log_probs(logits, targets, vocab, softcap=15.0, ignore_index=-1, *, 
         logp, ent = _SoftcapLogProbs.apply(flat, t, vocab, float(softcap), ignore_index, entropy)
     else:
         logp, ent = _eager_log_probs(flat, t, vocab, softcap, ignore_index)
-    return (logp.view(targets.shape), ent.view(targets.shape)) if entropy else logp.view(targets.shape)
+    if targets.ndim != 1:
+        logp, ent = logp.view(targets.shape), ent.view(targets.shape) if entropy else None
+    return (logp, ent) if entropy else logp
 
 
 class PolicyLoss(NamedTuple):
@@ -363,7 +383,7 @@ def policy_loss(logits, targets, old_log_probs, advantages, vocab, softcap=15.0,
             loss, logp, stats = _PolicyLossFused.apply(*args, float(expected_grad))
         else:
             loss, logp, stats = _PolicyLoss.apply(*args, grad)
-        return PolicyLoss(loss, logp.view(targets.shape), stats[0], stats[1])
+        return PolicyLoss(loss, logp if targets.ndim == 1 else logp.view(targets.shape), *stats.unbind(0))
     if w is not None:
         t = torch.where(w != 0, t, ignore_index)
     keep = t != ignore_index

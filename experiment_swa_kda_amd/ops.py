@@ -13,6 +13,7 @@ rmsnorm_gate.cu:277-284).
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -782,7 +783,11 @@ def rescale_bf16_if_changed(data, actual, expected):
     _check_dtype("rescale_bf16_if_changed", data, torch.bfloat16, "data")
     if not data.is_contiguous():
         raise RuntimeError("rescale_bf16_if_changed: data must be contiguous")
-    actual = actual.to(torch.float32).reshape(1).contiguous()
+    return _rescale_bf16_if_changed(dev, data, actual.to(torch.float32).reshape(1).contiguous(), expected)
+
+
+def _rescale_bf16_if_changed(dev, data, actual, expected):
+    """rescale_bf16_if_changed on checked operands."""
     with _on(dev):
         rc = _lib.load().kda_bf16_rescale_if_changed(data.numel(), ptr(data), ptr(actual), float(expected),
                                                      _stream(dev))
@@ -814,12 +819,13 @@ _LORA_ROW_IDS = 1024  # the most rows of own ids that the adapters' kernels take
 
 def _lora_way(M, K, N):
     """How a contraction of K with its adapters runs best on M rows and N outputs: as one kernel, or the
-    adapters' part alone with a library product added to it.  One kernel takes 22 us against 43 for M 8192,
-    K 384, N 1536, 21 / 28 for 8192 x 768 x 768, 12 / 21 for 2048 x 384 x 1536, 21 / 27 for 8192 x 1536 x 384,
-    but 20 / 17 for 2048 x 1536 x 384 (48 tiles), 79 / 71 for the transposed 8192 x 4096 x 1024 and 163 / 111
-    for 7777 x 4096 x 2048 (the library's larger tiles read their operands half as often)."""
-    whole = K <= 768 or (K <= 1536 and N <= 1024 and -(-M // 128) * -(-N // 128) >= 128)
-    return KDA_LORA_WHOLE if whole else KDA_LORA_PART
+    adapters' part alone with a library product added to it (whose call takes the host 10 us more).  Rank
+    16, one kernel / the part way, us: 22 / 43 for M 8192, K 384, N 1536; 21 / 27 for 8192 x 1536 x 384;
+    33 / 38 for 8192 x 2048 x 512; 18 / 21 for 512 x 1024 x 4096; 39 / 43 for 2048 x 384 x 8192; but 132 / 107
+    for 8192 x 384 x 8192, 62 / 53 for 8192 x 1024 x 2048, 209 / 131 for 8192 x 768 x 8192 and 41 / 23 for 128 x
+    4096 x 1024: the library's tiles are larger, which pays over many steps of many tiles."""
+    tiles = -(-M // 128) * -(-N // 128)
+    return KDA_LORA_WHOLE if K <= 2048 and tiles * K <= 1 << 19 else KDA_LORA_PART
 
 
 def _lora_check(what, x, w16, a, b, ids, scale):
@@ -843,7 +849,11 @@ def lora_forward(x, w16, a, b, ids, scale):
     [n] f32.  u [3, M, R] = scale_a x A_a^T as three bf16 parts whose sum is the f32 value.  y is rounded
     once; where the library multiplies x W^T (:func:`_lora_way`), the adapters' part once before."""
     dev, per = _lora_check("lora_forward", x, w16, a, b, ids, scale)
-    x, w16, a, b, scale = _c(x), _c(w16), _c(a), _c(b), _c(scale)
+    return _lora_forward(dev, per, _c(x), _c(w16), _c(a), _c(b), ids, _c(scale))
+
+
+def _lora_forward(dev, per, x, w16, a, b, ids, scale):
+    """lora_forward on checked and contiguous operands, ids for ``per`` rows each."""
     (M, K), N, (n, R) = x.shape, w16.shape[0], a.shape[:2]
     u = torch.empty(3, M, R, dtype=torch.bfloat16, device=dev)
     y = torch.empty(M, N, dtype=torch.bfloat16, device=dev)
@@ -872,17 +882,22 @@ def lora_backward(x, w16, a, b, ids, scale, u, grad, need_x, need_a, need_b):
     if grad.shape != (M, N) or u.shape != (3, M, R) or u.dtype != torch.bfloat16 or {grad.device, u.device} != {dev}:
         raise RuntimeError(f"{what}: grad [M, N] and u [3, M, R] expected")
     x, w16, a, b, scale, u, grad = (_c(t) for t in (x, w16, a, b, scale, u, grad))
+    return _lora_backward(dev, per, x, w16, a, b, ids, scale, u, grad, need_x, need_a, need_b)
+
+
+def _lora_backward(dev, per, x, w16, a, b, ids, scale, u, grad, need_x, need_a, need_b):
+    """lora_backward on checked and contiguous operands (on autograd's thread, which wakes up for it, a
+    check costs twice what it does elsewhere)."""
+    (M, K), N, (n, R) = x.shape, w16.shape[0], a.shape[:2]
     lib = _lib.load()
     how = _lora_way(M, N, K)
-    t = torch.empty_like(u) if need_x or need_a else None
     dx = torch.empty_like(x) if need_x else None
     da = torch.empty(n, R, K, dtype=torch.float32, device=dev) if need_a else None
     db = torch.empty(n, N, R, dtype=torch.float32, device=dev) if need_b else None
     scratch = torch.empty(lib.kda_lora_backward_scratch_bytes(M, N, K, R, n), dtype=torch.uint8, device=dev)
     with _on(dev):
         rc = lib.kda_lora_backward(M, N, K, R, n, ptr(ids), per, ptr(x), K, ptr(grad), N, ptr(w16), ptr(a), ptr(b),
-                                   ptr(scale), ptr(u), how, ptr(t), ptr(dx), ptr(da), ptr(db), ptr(scratch),
-                                   _stream(dev))
+                                   ptr(scale), ptr(u), how, ptr(dx), ptr(da), ptr(db), ptr(scratch), _stream(dev))
         check(rc, "kda_lora_backward")
         if need_x and how == KDA_LORA_PART:
             dx.addmm_(grad, w16)
@@ -952,6 +967,11 @@ def softcap_log_probs_backward(logits, targets, lse, entropy, g, h, vocab, softc
     logits, targets, lse, entropy, g, h = (_c(t) for t in (logits, targets, lse, entropy, g, h))
     if scale is not None:
         scale = scale.to(device=dev, dtype=torch.float32).reshape(1).contiguous()
+    return _softcap_log_probs_backward(dev, logits, targets, lse, entropy, g, h, vocab, softcap, ignore_index, scale)
+
+
+def _softcap_log_probs_backward(dev, logits, targets, lse, entropy, g, h, vocab, softcap, ignore_index, scale):
+    """softcap_log_probs_backward on checked and contiguous operands."""
     rows, stride = logits.shape
     grad = torch.empty_like(logits)
     with _on(dev):
@@ -986,6 +1006,7 @@ def policy_rows(targets, log_probs, old_log_probs, advantages, ref_log_probs, we
     return loss, stats, slope
 
 
+@functools.lru_cache
 def policy_fused_supported(stride):
     """True where the one-pass policy loss takes rows of this many columns (at most 32768)."""
     return bool(_lib.load().kda_policy_fused_supported(int(stride)))

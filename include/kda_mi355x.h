@@ -662,9 +662,8 @@ int kda_lora_grad(int64_t M, int32_t J, int32_t R, int32_t n, const int32_t* ids
  * KDA_LORA_PART, which leaves the adapters' part alone in y or dx for the caller to add the shared
  * product to (weight is then not read).  x rows have stride ldx, grad_output [M, N] rows ldg.
  *   forward   u [3, M, R] and y [M, N]
- *   backward  t [3, M, R] = scale B^T dy (scratch of the caller's, also for da alone), and of dx
- *             [M, K] bf16, da [n, R, K] and db [n, N, R] f32 those that are not NULL (dx, da need t; db
- *             needs the forward's u)
+ *   backward  of dx [M, K] bf16, da [n, R, K] and db [n, N, R] f32 those that are not NULL (db from
+ *             the forward's u); scratch of kda_lora_backward_scratch_bytes
  */
 #define KDA_LORA_ROWS 0
 #define KDA_LORA_WHOLE 1
@@ -677,7 +676,7 @@ size_t kda_lora_backward_scratch_bytes(int64_t M, int32_t N, int32_t K, int32_t 
 int kda_lora_backward(int64_t M, int32_t N, int32_t K, int32_t R, int32_t n, const int32_t* ids,
                       int64_t rows_per_id, const void* x, int64_t ldx, const void* grad_output, int64_t ldg,
                       const void* weight, const void* lora_a, const void* lora_b, const float* scale,
-                      const void* u, int32_t how, void* t, void* dx, float* da, float* db, void* scratch,
+                      const void* u, int32_t how, void* dx, float* da, float* db, void* scratch,
                       hipStream_t stream);
 
 /*

@@ -175,7 +175,7 @@ def test_c_abi_refuses_bad_calls_without_gpu():
     refused(linear(4, 16, 16, 8, 2, p, 1, p, 16, p, 0, None, p, p, None), "null")
     refused(forward(4, 16, 32, 8, 2, p, 1, p, 32, p, p, p, p, 3, p, p, None), "unknown way")
     refused(forward(65, 16, 32, 8, 2, p, 1, p, 32, p, p, p, p, 0, p, p, None), "at most 64 rows")
-    refused(backward(4, 16, 32, 8, 2, p, 1, p, 32, p, 16, p, p, p, p, p, 0, p, p, p, p, p, None), "unknown way")
-    refused(backward(4, 16, 32, 8, 2, p, 1, p, 32, p, 16, p, p, p, p, p, 1, None, p, p, p, p, None), "null")
+    refused(backward(4, 16, 32, 8, 2, p, 1, p, 32, p, 16, p, p, p, p, p, 0, p, p, p, p, None), "unknown way")
+    refused(backward(4, 16, 32, 8, 2, p, 1, p, 32, p, 16, p, p, p, p, p, 1, p, p, p, None, None), "null")
     assert lib.kda_lora_grad_scratch_bytes(32, 128, 16, 4) == 0  # one range is the result itself
     assert lib.kda_lora_grad_scratch_bytes(8192, 128, 16, 4) > 0
