@@ -49,7 +49,68 @@ __device__ __forceinline__ bf16x8 gl_col_frag(const char* part, int c0, int lane
   return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+// Adds the adapters of a wave's 64 rows from mw on, one after another, to its columns from nw on.
 template <bool WT>
+__device__ __forceinline__ void gl_add_adapters(LoraRows rows, int N, int R, const bf16* __restrict__ u,
+                                                const bf16* __restrict__ f, int mw, int nw, int lane,
+                                                bf16* piece, f32x4 (&acc)[4][4]) {
+  const int lr = lane % 16, kg = lane / 16;
+  const int row_id = rows.id(mw + lane);
+  const size_t plane = (size_t)rows.M * R;
+  // (buffers from the wave's first row or column: 32-bit offsets, and what is outside reads as zero)
+  const __amdgpu_buffer_rsrc_t rhi = raw_rsrc(u + (size_t)mw * R), rlo = raw_rsrc(u + plane + (size_t)mw * R);
+  int a = next_adapter(row_id, -1), r0 = 0;
+  while (a != kNoAdapter) {
+    const int r = r0 + 8 * kg;
+    const size_t base = (size_t)a * R * N;
+    bf16x8 ff[4];
+    if constexpr (WT) {
+      const __amdgpu_buffer_rsrc_t rf = raw_rsrc(f + base + (size_t)r0 * N + nw);
+      const int rr = lane / 4, c = 8 * (lane % 4);
+      bf16x8 v[2][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)  // 32 rows of 32 columns
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          v[h][i] = buffer8(rf, r0 + 16 * i + rr < R && nw + 32 * h + c < N ? (rr * N + c) * 2 : kDropOffset, 32 * i * N + 64 * h);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < 2; ++i) *(bf16x8*)(piece + (16 * i + rr) * kGlPiecePitch + c) = v[h][i];
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int c2 = 0; c2 < 2; ++c2) ff[2 * h + c2] = lds_col_frag(piece, kGlPiecePitch, 0, 16 * c2, lane);
+      }
+    } else {
+      const __amdgpu_buffer_rsrc_t rf = raw_rsrc(f + base + (size_t)nw * R);
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        ff[c] = buffer8(rf, r < R && nw + 16 * c + lr < N ? (lr * R + r) * 2 : kDropOffset, 32 * c * R);
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const bool mine = __shfl(row_id, 16 * t + lr) == a;
+      const int off = r < R && mw + 16 * t + lr < rows.M ? (lr * R + r) * 2 : kDropOffset;
+      const bf16x8 hi = buffer8(rhi, off, 32 * t * R), lo = buffer8(rlo, off, 32 * t * R);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        // (chosen, not multiplied by zero: an infinity in this adapter stays out of other rows)
+        const f32x4 d = mfma16(ff[c], lo, mfma16(ff[c], hi, zero4()));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[c][t][i] += mine ? d[i] : 0.f;
+      }
+      __builtin_amdgcn_sched_barrier(0);  // (all rows at once would spill registers)
+    }
+    r0 += kGlDepth;
+    if (r0 >= R) {
+      r0 = 0;
+      a = next_adapter(row_id, a);
+    }
+  }
+}
+
+template <bool WT, bool FIRST>
 __global__ __launch_bounds__(kGlThreads, 3) void lora_linear_kernel(LoraRows rows, int N, int K, int R,
                                                                     const bf16* __restrict__ x, long ldx,
                                                                     const bf16* __restrict__ w,
@@ -134,64 +195,8 @@ __global__ __launch_bounds__(kGlThreads, 3) void lora_linear_kernel(LoraRows row
 #pragma unroll
     for (int t = 0; t < 4; ++t) acc[c][t] = zero4();
 
-  // ---- first, while the loaders' first steps are on their way, the adapters of the wave's 64 rows, one
-  // after another ----
-  {
-    const int row_id = rows.id(mw + lane);
-    const size_t plane = (size_t)rows.M * R;
-    // (buffers from the wave's first row or column: 32-bit offsets, and what is outside reads as zero)
-    const __amdgpu_buffer_rsrc_t rhi = raw_rsrc(u + (size_t)mw * R), rlo = raw_rsrc(u + plane + (size_t)mw * R);
-    int a = next_adapter(row_id, -1), r0 = 0;
-    while (a != kNoAdapter) {
-      const int r = r0 + 8 * kg;
-      const size_t base = (size_t)a * R * N;
-      bf16x8 ff[4];
-      if constexpr (WT) {
-        const __amdgpu_buffer_rsrc_t rf = raw_rsrc(f + base + (size_t)r0 * N + nw);
-        const int rr = lane / 4, c = 8 * (lane % 4);
-        bf16x8 v[2][2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)  // 32 rows of 32 columns
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            v[h][i] = buffer8(rf, r0 + 16 * i + rr < R && nw + 32 * h + c < N ? (rr * N + c) * 2 : kDropOffset, 32 * i * N + 64 * h);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          asm volatile("" ::: "memory");
-#pragma unroll
-          for (int i = 0; i < 2; ++i) *(bf16x8*)(piece[wave] + (16 * i + rr) * kGlPiecePitch + c) = v[h][i];
-          asm volatile("" ::: "memory");
-#pragma unroll
-          for (int c2 = 0; c2 < 2; ++c2) ff[2 * h + c2] = lds_col_frag(piece[wave], kGlPiecePitch, 0, 16 * c2, lane);
-        }
-      } else {
-        const __amdgpu_buffer_rsrc_t rf = raw_rsrc(f + base + (size_t)nw * R);
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          ff[c] = buffer8(rf, r < R && nw + 16 * c + lr < N ? (lr * R + r) * 2 : kDropOffset, 32 * c * R);
-      }
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const bool mine = __shfl(row_id, 16 * t + lr) == a;
-        const int off = r < R && mw + 16 * t + lr < rows.M ? (lr * R + r) * 2 : kDropOffset;
-        const bf16x8 hi = buffer8(rhi, off, 32 * t * R), lo = buffer8(rlo, off, 32 * t * R);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          // (chosen, not multiplied by zero: an infinity in this adapter stays out of other rows)
-          const f32x4 d = mfma16(ff[c], lo, mfma16(ff[c], hi, zero4()));
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[c][t][i] += mine ? d[i] : 0.f;
-        }
-        __builtin_amdgcn_sched_barrier(0);  // (all rows at once would spill registers)
-      }
-      r0 += kGlDepth;
-      if (r0 >= R) {
-        r0 = 0;
-        a = next_adapter(row_id, a);
-      }
-    }
-  }
-
+  // (while the loaders' first steps are on their way)
+  if constexpr (FIRST) gl_add_adapters<WT>(rows, N, R, u, f, mw, nw, lane, piece[WT ? wave : 0], acc);
   ring_barrier();  // B0
   for (int q = 0; q < nsteps; ++q) {
     const char* st = smem + (q % kGlStages) * kGlStage;
@@ -206,6 +211,13 @@ __global__ __launch_bounds__(kGlThreads, 3) void lora_linear_kernel(LoraRows row
 #pragma unroll
       for (int t = 0; t < 4; ++t) acc[c][t] = mfma16(fw[c], fx[t], acc[c][t]);
     ring_barrier();  // A(q)
+  }
+  if constexpr (!FIRST) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) asm volatile("" : "+v"(acc[c][t]));  // (one loop's results, the next one's start: no copies)
+    gl_add_adapters<WT>(rows, N, R, u, f, mw, nw, lane, piece[WT ? wave : 0], acc);
   }
 
   // accumulator: column 16 c + 4 kg + i, row 16 t + lr of the wave's 64; through the wave's half stage
@@ -251,7 +263,14 @@ extern "C" int kda_lora_linear(int64_t M, int32_t N, int32_t K, int32_t R, int32
     hipLaunchKernelGGL(kern, dim3(grid), dim3(kGlThreads), 0, stream, rows, N, K, R, (const bf16*)x, (long)ldx,
                        (const bf16*)weight, (const bf16*)u, (const bf16*)factor, (bf16*)y, (int)tiles_n, (int)items);
   };
-  weight_rows ? go(lora_linear_kernel<true>) : go(lora_linear_kernel<false>);
+  // One round of tiles (two workgroups a CU) adds the adapters while its first loads are on their way (8192 x
+  // 1536 -> 384 20.9 us against 22.0); of several rounds one tile's adapters hide behind another's steps, and
+  // come last, when the loads of the tile after are long under way (512 x 384 -> 32768 29.7 / 33.5, 8192 x 384
+  // -> 4096 50 / 55).
+  if (items <= 2 * 256)
+    weight_rows ? go(lora_linear_kernel<true, true>) : go(lora_linear_kernel<false, true>);
+  else
+    weight_rows ? go(lora_linear_kernel<true, false>) : go(lora_linear_kernel<false, false>);
   KDA_LAUNCH_CHECK("lora_linear");
   return KDA_OK;
 }

@@ -820,12 +820,12 @@ _LORA_ROW_IDS = 1024  # the most rows of own ids that the adapters' kernels take
 def _lora_way(M, K, N):
     """How a contraction of K with its adapters runs best on M rows and N outputs: as one kernel, or the
     adapters' part alone with a library product added to it (whose call takes the host 10 us more).  Rank
-    16, one kernel / the part way, us: 22 / 43 for M 8192, K 384, N 1536; 21 / 27 for 8192 x 1536 x 384;
-    33 / 38 for 8192 x 2048 x 512; 18 / 21 for 512 x 1024 x 4096; 39 / 43 for 2048 x 384 x 8192; but 132 / 107
-    for 8192 x 384 x 8192, 62 / 53 for 8192 x 1024 x 2048, 209 / 131 for 8192 x 768 x 8192 and 41 / 23 for 128 x
-    4096 x 1024: the library's tiles are larger, which pays over many steps of many tiles."""
+    16, one kernel / the part way, us: 22 / 43 for M 8192, K 384, N 1536; 399 / 512 for 8192 x 384 x 32768;
+    462 / 554 for 8192 x 512 x 32768; 27 / 38 for 8192 x 2048 x 512; 19 / 21 for 512 x 1024 x 4096; but 56 / 52
+    for 8192 x 1024 x 2048, 179 / 137 for 8192 x 768 x 8192 and 42 / 23 for 128 x 4096 x 1024: the library's
+    tiles are larger, which pays over many steps of many tiles."""
     tiles = -(-M // 128) * -(-N // 128)
-    return KDA_LORA_WHOLE if K <= 2048 and tiles * K <= 1 << 19 else KDA_LORA_PART
+    return KDA_LORA_WHOLE if K <= 512 or (K <= 2048 and tiles * K <= 1 << 19) else KDA_LORA_PART
 
 
 def _lora_check(what, x, w16, a, b, ids, scale):
