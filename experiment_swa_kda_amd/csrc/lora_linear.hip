@@ -281,7 +281,7 @@ extern "C" int kda_lora_forward(int64_t M, int32_t N, int32_t K, int32_t R, int3
                                 void* y, hipStream_t stream) {
   KDA_REQUIRE(how >= KDA_LORA_ROWS && how <= KDA_LORA_PART, "lora_forward: unknown way");
   if (how == KDA_LORA_ROWS) {
-    KDA_REQUIRE(M >= 0 && M <= 64, "lora_forward: at most 64 rows");
+    KDA_REQUIRE(M >= 0 && M <= 512, "lora_forward: at most 512 rows");
     return kda_lora_linear_rows((int32_t)M, N, K, R, n, ids, rows_per_id, x, ldx, weight, lora_a, lora_b, scale, u, y,
                                 stream);
   }

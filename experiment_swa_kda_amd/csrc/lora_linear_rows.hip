@@ -123,7 +123,7 @@ extern "C" int kda_lora_linear_rows(int32_t rows, int32_t out_dim, int32_t in_di
                                     const void* weight, const void* lora_a, const void* lora_b, const float* scale,
                                     void* u, void* y, hipStream_t stream) {
   using namespace kda;
-  KDA_REQUIRE(rows >= 0 && rows <= 64, "lora_linear_rows: at most 64 rows");
+  KDA_REQUIRE(rows >= 0 && rows <= 512, "lora_linear_rows: at most 512 rows");
   KDA_REQUIRE(out_dim > 0 && out_dim % 8 == 0, "lora_linear_rows: out_dim must be a multiple of 8");
   int rc = check_lora("lora_linear_rows", rows, in_dim, R, n, ids, rows_per_id);
   if (rc != KDA_OK) return rc;

@@ -105,8 +105,8 @@ struct TokSum {
 
 // logp, lse and entropy of a row from its sums se = sum e^z, sz = sum z e^z, and its target's logit.
 // Formed in 64 bits from f32 pieces that are small, so that none loses what an f32 lse of 10 would:
-// lse = k log 2 + log m with se = m 2^k, m around 1; z_y = cap (1 - d), d = 2 / (1 + e^(2|a|)),
-// where |tanh| is over a half.  Sequence sums and their differences then keep 1e-7 of a row.
+// lse = k log 2 + log m with se = m 2^k, m around 1; z_y = cap (1 - d), d = 2 / (1 + e^(2|a|)), for |a| of 4
+// and more.  Sequence sums and their differences then keep 1e-7 of a row.
 __device__ __forceinline__ double tok_lse(float se) {
   int k;
   float m = frexpf(se, &k);  // [0.5, 1)
@@ -116,9 +116,23 @@ __device__ __forceinline__ double tok_lse(float se) {
   }
   return (double)k * 0.69314718055994530942 + (double)logf(m);
 }
+// (f32's tanh would leave a z of 5 up to 2^-21 off, most of a row's error; Lambert's continued fraction
+// tanh a = a / (1 + a^2 / (3 + a^2 / (5 + ...))), ten levels of it by its recurrence, is within 1e-9 for
+// |a| < 4, and beyond that d is small)
 __device__ __forceinline__ double tok_z(float raw, float cap) {
-  const float a = fabsf(raw) / cap, t = tanhf(a);
-  const double z = t < 0.5f ? (double)cap * t : (double)cap * (1.0 - (double)(2.f / (1.f + expf(2.f * a))));
+  const double a = (double)raw / (double)cap, b = a * a;
+  double p0 = 1.0, p1 = 1.0, q0 = 0.0, q1 = 1.0;
+#pragma unroll 1
+  for (int k = 3; k <= 21; k += 2) {
+    const double p = fma(b, p0, k * p1), q = fma(b, q0, k * q1);
+    p0 = p1;
+    p1 = p;
+    q0 = q1;
+    q1 = q;
+  }
+  const float m = fabsf(raw) / cap;
+  const double far = (double)cap * (1.0 - (double)(2.f / (1.f + expf(2.f * m))));
+  const double z = m < 4.f ? (double)cap * fabs(a) * q1 / p1 : far;
   return raw < 0.f ? -z : raw != raw ? (double)raw : z;
 }
 
@@ -391,8 +405,9 @@ struct PolicyTerm {
   bool clipped;
 };
 
-__device__ __forceinline__ PolicyTerm policy_term(const PolicyArgs& a, float logp, float old, float adv, float ref) {
-  const float ratio = expf(logp - old);
+// (the log-probability in 64 bits: rounded first, a value of 10 would leave its difference 2^-21 off)
+__device__ __forceinline__ PolicyTerm policy_term(const PolicyArgs& a, double logp, float old, float adv, float ref) {
+  const float ratio = expf((float)(logp - old));
   const float free_ = adv == 0.f ? 0.f : ratio * adv;  // an infinite ratio of no advantage counts nothing
   const float held = fminf(fmaxf(ratio, a.lo), a.hi) * adv;
   PolicyTerm t;
@@ -401,7 +416,7 @@ __device__ __forceinline__ PolicyTerm policy_term(const PolicyArgs& a, float log
   t.slope = t.clipped ? 0.f : -free_;
   t.kl = 0.f;
   if (a.ref_logp) {
-    const float d = ref - logp, em = expm1f(d);
+    const float d = (float)(ref - logp), em = expm1f(d);
     t.kl = em - d;
     if (a.kl_coef != 0.f) {
       t.loss += a.kl_coef * t.kl;
@@ -629,9 +644,10 @@ __global__ __launch_bounds__(THREADS, 4) void policy_fused_kernel(
       const long rl = at(lane);
       float logp = 0.f;
       if (s_col[lane] != kRowOff) {
-        logp = (float)(s_z[lane] - tok_lse(s_sum[lane]));
+        const double lp = s_z[lane] - tok_lse(s_sum[lane]);
+        logp = (float)lp;
         const double w = pa.weights ? pa.weights[rl] : 1.f;
-        const PolicyTerm t = policy_term(pa, logp, pa.old_logp[rl], pa.adv[rl], pa.ref_logp ? pa.ref_logp[rl] : 0.f);
+        const PolicyTerm t = policy_term(pa, lp, pa.old_logp[rl], pa.adv[rl], pa.ref_logp ? pa.ref_logp[rl] : 0.f);
         s_acc[0][lane] += w * t.loss;
         s_acc[1][lane] += w * t.kl;
         s_acc[2][lane] += t.clipped ? w : 0.0;
@@ -669,7 +685,7 @@ constexpr int kRowsThreads = 1024;
 constexpr int kRowsAhead = 4;  // rows of a thread whose loads are in flight together
 __global__ __launch_bounds__(kRowsThreads) void policy_rows_kernel(long rows, const int64_t* __restrict__ targets,
                                                                    int64_t ignore_index,
-                                                                   const float* __restrict__ logp_row, PolicyArgs a,
+                                                                   const double* __restrict__ logp_row, PolicyArgs a,
                                                                    float* __restrict__ loss, float* __restrict__ stats,
                                                                    float* __restrict__ slope_row) {
   __shared__ double red[3][kRowsThreads / kWave];
@@ -694,7 +710,8 @@ __global__ __launch_bounds__(kRowsThreads) void policy_rows_kernel(long rows, co
   }
   double sl = 0.0, sk = 0.0, sc = 0.0;
   for (long r0 = threadIdx.x; r0 < rows; r0 += kRowsAhead * kRowsThreads) {
-    float w[kRowsAhead], lp[kRowsAhead], old[kRowsAhead], adv[kRowsAhead], ref[kRowsAhead];
+    float w[kRowsAhead], old[kRowsAhead], adv[kRowsAhead], ref[kRowsAhead];
+    double lp[kRowsAhead];
     bool on[kRowsAhead];
 #pragma unroll
     for (int q = 0; q < kRowsAhead; ++q) {  // all loads before any is used
@@ -901,17 +918,17 @@ extern "C" int kda_softcap_log_probs_backward(int64_t rows, int32_t vocab, int64
   return KDA_OK;
 }
 
-extern "C" int kda_policy_rows(int64_t rows, const int64_t* targets, int64_t ignore_index, const float* log_probs,
+extern "C" int kda_policy_rows(int64_t rows, const int64_t* targets, int64_t ignore_index, const double* log_probs64,
                                const float* old_log_probs, const float* advantages, const float* ref_log_probs,
                                const float* weights, float clip_lo, float clip_hi, float kl_coef, float* loss,
                                float* stats, float* slope_rows, hipStream_t stream) {
   using namespace kda;
   KDA_REQUIRE(rows >= 0 && rows <= 0x7fffffff, "policy_rows: invalid row count");
-  KDA_REQUIRE(loss && stats && (rows == 0 || (targets && log_probs && old_log_probs && advantages)), "policy_rows: null pointer");
+  KDA_REQUIRE(loss && stats && (rows == 0 || (targets && log_probs64 && old_log_probs && advantages)), "policy_rows: null pointer");
   KDA_REQUIRE(clip_lo <= 1.f && clip_hi >= 1.f, "policy_rows: the clipping range must hold 1");
   const PolicyArgs a{old_log_probs, advantages, ref_log_probs, weights, clip_lo, clip_hi, kl_coef};
   hipLaunchKernelGGL(policy_rows_kernel, dim3(1), dim3(kRowsThreads), 0, stream, (long)rows, targets, ignore_index,
-                     log_probs, a, loss, stats, slope_rows);
+                     log_probs64, a, loss, stats, slope_rows);
   KDA_LAUNCH_CHECK("policy_rows");
   return KDA_OK;
 }

@@ -223,8 +223,8 @@ class _PolicyLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, old, adv, ref, weights, vocab, softcap, ignore_index, lo, hi, kl_coef, grad):
         logits, targets = ops._c(logits), ops._c(targets)
-        logp, lse, _ = ops.softcap_log_probs_forward(logits, targets, vocab, softcap, ignore_index)
-        loss, stats, slope = ops.policy_rows(targets, logp, old, adv, ref, weights, lo, hi, kl_coef, ignore_index,
+        logp, lse, _, logp64 = ops.softcap_log_probs_forward(logits, targets, vocab, softcap, ignore_index, double=True)
+        loss, stats, slope = ops.policy_rows(targets, logp64, old, adv, ref, weights, lo, hi, kl_coef, ignore_index,
                                              slopes=grad)
         ctx.save_for_backward(logits, targets, lse, slope)
         ctx.args = (vocab, softcap, ignore_index)
@@ -280,7 +280,7 @@ class _PreferenceLoss(torch.autograd.Function):
     def forward(ctx, logits, targets, pairs, seq_len, cu_seqlens, ref, vocab, softcap, ignore_index, beta, smoothing,
                 average, grad):
         logits, targets = ops._c(logits), ops._c(targets)
-        logp, lse, _ = ops.softcap_log_probs_forward(logits, targets, vocab, softcap, ignore_index, double=True)
+        _, lse, _, logp = ops.softcap_log_probs_forward(logits, targets, vocab, softcap, ignore_index, double=True)
         loss, seq, margins, slope = ops.preference_pairs(targets, logp, pairs, seq_len, cu_seqlens, ref, beta,
                                                          smoothing, average, ignore_index, slopes=grad)
         ctx.save_for_backward(logits, targets, lse, slope)

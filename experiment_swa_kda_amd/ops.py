@@ -813,8 +813,17 @@ def embedding_backward(idx, grad_output, vocab):
     return dw
 
 
-_LORA_ROWS = 64  # the most rows kda_lora_linear_rows takes
+_LORA_ROWS = 512  # the most rows kda_lora_linear_rows takes
 _LORA_ROW_IDS = 1024  # the most rows of own ids that the adapters' kernels take one by one
+
+
+def _lora_few(M, K, N, per):
+    """Whether the kernel of few rows takes a call of ids for ``per`` rows each: up to 512 rows with ids of
+    their own, 256 otherwise, while each workgroup's read of all rows stays small.  Rank 16, an adapter each,
+    this kernel / the part way, us: M 256 9.5 / 12 for 384 -> 1536 and 20 / 20 for 2048 -> 2048, M 512 15 / 17 and
+    33 / 25, M 32 and 64 16 / 17 and 31 / 24 for 384 -> 32768; sequences as one kernel: M 256 11, M 512 11.5 for
+    384 -> 1536."""
+    return M <= (_LORA_ROWS if per == 1 else _LORA_ROWS // 2) and M * N <= 1 << 20 and M * N * K <= 1 << 30
 
 
 def _lora_way(M, K, N):
@@ -857,7 +866,7 @@ def _lora_forward(dev, per, x, w16, a, b, ids, scale):
     (M, K), N, (n, R) = x.shape, w16.shape[0], a.shape[:2]
     u = torch.empty(3, M, R, dtype=torch.bfloat16, device=dev)
     y = torch.empty(M, N, dtype=torch.bfloat16, device=dev)
-    if M <= _LORA_ROWS:
+    if _lora_few(M, K, N, per):
         how = KDA_LORA_ROWS
     elif per == 1 and M <= _LORA_ROW_IDS:
         how = KDA_LORA_PART  # (one kernel's tiles of as many adapters as rows: M 256, K 384, N 1536 85 us, this 12)
@@ -940,21 +949,22 @@ def _check_rows(what, targets, *rows):
 
 def softcap_log_probs_forward(logits, targets, vocab, softcap, ignore_index=-1, *, entropy=False, double=False):
     """logits [rows, stride] bf16 (stride >= vocab), targets [rows] int64 -> (log-probabilities f32
-    [rows], with ``double`` f64, lse f32 [rows], entropies f32 [rows] or None); zeros in the rows
-    whose target is ignore_index, which are not read."""
+    [rows], lse f32 [rows], entropies f32 [rows] or None, and with ``double`` the log-probabilities in
+    f64); zeros in the rows whose target is ignore_index, which are not read."""
     what = "softcap_log_probs_forward"
     dev = _token_inputs(what, logits, targets)
     logits, targets = _c(logits), _c(targets)
     rows, stride = logits.shape
-    logp = torch.empty(rows, dtype=torch.float64 if double else torch.float32, device=dev)
+    logp = torch.empty(rows, dtype=torch.float32, device=dev)
+    logp64 = torch.empty(rows, dtype=torch.float64, device=dev) if double else None
     lse = torch.empty(rows, dtype=torch.float32, device=dev)
     ent = torch.empty(rows, dtype=torch.float32, device=dev) if entropy else None
     with _on(dev):
         rc = _lib.load().kda_softcap_log_probs_forward(
             rows, int(vocab), stride, float(softcap), ptr(logits), ptr(targets), int(ignore_index),
-            None if double else ptr(logp), ptr(logp) if double else None, ptr(lse), ptr(ent), _stream(dev))
+            ptr(logp), ptr(logp64), ptr(lse), ptr(ent), _stream(dev))
     check(rc, "kda_softcap_log_probs_forward")
-    return logp, lse, ent
+    return (logp, lse, ent, logp64) if double else (logp, lse, ent)
 
 
 def softcap_log_probs_backward(logits, targets, lse, entropy, g, h, vocab, softcap, ignore_index=-1, *, scale=None):
@@ -982,24 +992,25 @@ def _softcap_log_probs_backward(dev, logits, targets, lse, entropy, g, h, vocab,
     return grad
 
 
-def policy_rows(targets, log_probs, old_log_probs, advantages, ref_log_probs, weights, clip_lo, clip_hi, kl_coef,
+def policy_rows(targets, log_probs64, old_log_probs, advantages, ref_log_probs, weights, clip_lo, clip_hi, kl_coef,
                 ignore_index=-1, *, slopes=False):
-    """Clipped policy loss of f32 row log-probabilities -> (loss, stats [2] = (KL, weight of the
+    """Clipped policy loss of f64 row log-probabilities -> (loss, stats [2] = (KL, weight of the
     clipped rows), d loss / d log_probs [rows] or None)."""
     what = "policy_rows"
-    dev = _require_cuda(what, targets, log_probs, old_log_probs, advantages, ref_log_probs, weights)
+    dev = _require_cuda(what, targets, log_probs64, old_log_probs, advantages, ref_log_probs, weights)
     _check_dtype(what, targets, torch.int64, "targets")
-    if targets.ndim != 1 or old_log_probs is None or advantages is None:
-        raise RuntimeError(f"{what}: targets, log_probs, old_log_probs and advantages [rows] expected")
-    _check_rows(what, targets, log_probs, old_log_probs, advantages, ref_log_probs, weights)
-    targets, log_probs, old_log_probs, advantages, ref_log_probs, weights = (
-        _c(t) for t in (targets, log_probs, old_log_probs, advantages, ref_log_probs, weights))
+    _check_dtype(what, log_probs64, torch.float64, "log_probs64")
+    if targets.ndim != 1 or log_probs64.shape != targets.shape or old_log_probs is None or advantages is None:
+        raise RuntimeError(f"{what}: targets, log_probs64, old_log_probs and advantages [rows] expected")
+    _check_rows(what, targets, old_log_probs, advantages, ref_log_probs, weights)
+    targets, log_probs64, old_log_probs, advantages, ref_log_probs, weights = (
+        _c(t) for t in (targets, log_probs64, old_log_probs, advantages, ref_log_probs, weights))
     loss = torch.empty((), dtype=torch.float32, device=dev)
     stats = torch.empty(2, dtype=torch.float32, device=dev)
-    slope = torch.empty_like(log_probs) if slopes else None
+    slope = torch.empty(targets.numel(), dtype=torch.float32, device=dev) if slopes else None
     with _on(dev):
         rc = _lib.load().kda_policy_rows(
-            targets.numel(), ptr(targets), int(ignore_index), ptr(log_probs), ptr(old_log_probs), ptr(advantages),
+            targets.numel(), ptr(targets), int(ignore_index), ptr(log_probs64), ptr(old_log_probs), ptr(advantages),
             ptr(ref_log_probs), ptr(weights), float(clip_lo), float(clip_hi), float(kl_coef), ptr(loss), ptr(stats),
             ptr(slope), _stream(dev))
     check(rc, "kda_policy_rows")

@@ -567,7 +567,7 @@ int kda_softcap_log_probs_backward(int64_t rows, int32_t vocab, int64_t stride, 
                                    hipStream_t stream);
 
 /*
- * Clipped policy loss of given log-probabilities (f32 [rows], as all row inputs):
+ * Clipped policy loss of given log-probabilities (f64 [rows]; the other row inputs f32):
  *   loss = sum_r w_r (-min(q_r A_r, clip(q_r, clip_lo, clip_hi) A_r) + kl_coef k_r),
  *   q = exp(log_probs - old_log_probs),  d = ref_log_probs - log_probs,  k = e^d - d - 1
  * (ref_log_probs NULL: k = 0), w_r = weights[r], or 1 / number of rows with a target (NULL).
@@ -575,7 +575,7 @@ int kda_softcap_log_probs_backward(int64_t rows, int32_t vocab, int64_t stride, 
  * (NULL: not written) = d loss / d log_probs.  Rows without a target or of weight 0 count
  * nothing.  Fixed-order f64 sums in one workgroup.
  */
-int kda_policy_rows(int64_t rows, const int64_t* targets, int64_t ignore_index, const float* log_probs,
+int kda_policy_rows(int64_t rows, const int64_t* targets, int64_t ignore_index, const double* log_probs64,
                     const float* old_log_probs, const float* advantages, const float* ref_log_probs,
                     const float* weights, float clip_lo, float clip_hi, float kl_coef, float* loss,
                     float* stats, float* slope_rows, hipStream_t stream);
@@ -635,7 +635,7 @@ int kda_lora_expand(int64_t M, int32_t J, int32_t R, int32_t n, const int32_t* i
                     const void* u, const void* factor, int32_t factor_cols, void* y, int64_t ldy,
                     hipStream_t stream);
 /*
- * The whole of y = x W^T + s B (A x) for at most 64 rows (out_dim a multiple of 8): weight
+ * The whole of y = x W^T + s B (A x) for at most 512 rows (out_dim a multiple of 8): weight
  * [out_dim, in_dim], lora_a [n, R, in_dim], lora_b [n, out_dim, R] bf16, rounded once; u [3, rows,
  * R] receives s A x.
  */

@@ -131,7 +131,7 @@ def test_another_requests_nan_and_an_unused_adapters_inf_stay_out(T):
 # contraction, outputs and rows of every way a call takes: few rows, rows with ids of their own, whole
 # sequences; one kernel for the projection or the adapters' part beside it, in either direction
 WAYS = [(6, 1, 64, 96), (9, 7, 1032, 72), (40, 1, 520, 4096), (90, 1, 64, 96), (6, 40, 64, 96), (6, 40, 1608, 72), (6, 40, 72, 1608),
-        (3, 90, 1600, 1544), (7, 190, 64, 200)]
+        (3, 90, 1600, 1544), (7, 190, 64, 200), (9, 60, 64, 200), (4, 75, 520, 4096)]
 
 
 @pytest.mark.parametrize("B,T,K,N", WAYS)

@@ -169,12 +169,12 @@ def test_c_abi_refuses_bad_calls_without_gpu():
     refused(grad(4, 16, 8, 2, p, 1, p, 16, None, 0, p, p, None), "null")
     refused(grad(4, 16, 8, 2, p, 1, p, 16, p, 0, None, p, None), "null")
     rows, linear, forward, backward = (getattr(lib, f"kda_lora_{k}") for k in ("linear_rows", "linear", "forward", "backward"))
-    refused(rows(65, 16, 32, 8, 2, p, 1, p, 32, p, p, p, p, p, p, None), "at most 64 rows")
+    refused(rows(513, 16, 32, 8, 2, p, 1, p, 32, p, p, p, p, p, p, None), "at most 512 rows")
     refused(rows(4, 12, 24, 8, 2, p, 1, p, 24, p, p, p, p, p, p, None), "out_dim must be a multiple of 8")
     refused(linear(4, 12, 16, 8, 2, p, 1, p, 16, p, 0, p, p, p, None), "multiples of 8")
     refused(linear(4, 16, 16, 8, 2, p, 1, p, 16, p, 0, None, p, p, None), "null")
     refused(forward(4, 16, 32, 8, 2, p, 1, p, 32, p, p, p, p, 3, p, p, None), "unknown way")
-    refused(forward(65, 16, 32, 8, 2, p, 1, p, 32, p, p, p, p, 0, p, p, None), "at most 64 rows")
+    refused(forward(513, 16, 32, 8, 2, p, 1, p, 32, p, p, p, p, 0, p, p, None), "at most 512 rows")
     refused(backward(4, 16, 32, 8, 2, p, 1, p, 32, p, 16, p, p, p, p, p, 0, p, p, p, p, None), "unknown way")
     refused(backward(4, 16, 32, 8, 2, p, 1, p, 32, p, 16, p, p, p, p, p, 1, p, p, p, None, None), "null")
     assert lib.kda_lora_grad_scratch_bytes(32, 128, 16, 4) == 0  # one range is the result itself
