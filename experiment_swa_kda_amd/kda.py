@@ -282,18 +282,18 @@ def _lora_linear(x, weight, a, b, ids, scaling, w16, a16, b16):
 
 def _check_lora(x, weight, a, b, ids, scaling):
     """The checks of lora_linear; returns ids as int32."""
-    K = x.shape[-1] if x.ndim else 0
-    if x.ndim < 2 or weight.ndim != 2 or weight.shape[1] != K:
+    xs, ws, fs = x.shape, weight.shape, a.shape
+    if len(xs) < 2 or len(ws) != 2 or ws[1] != xs[-1]:
         raise ValueError("lora_linear: x [..., K] and weight [N, K] expected")
-    if a.ndim != 3 or b.ndim != 3 or a.shape[0] != b.shape[0] or a.shape[2] != K or b.shape != (a.shape[0], weight.shape[0], a.shape[1]):
+    if len(fs) != 3 or fs[2] != xs[-1] or b.shape != (fs[0], ws[0], fs[1]):
         raise ValueError("lora_linear: lora_a [n, R, K] and lora_b [n, N, R] expected")
-    if scaling.shape != a.shape[:1]:
-        raise ValueError(f"lora_linear: scaling must have shape {tuple(a.shape[:1])}")
+    if scaling.shape != fs[:1]:
+        raise ValueError(f"lora_linear: scaling must have shape {tuple(fs[:1])}")
     if scaling.requires_grad and torch.is_grad_enabled():
         raise ValueError("lora_linear: scaling is a constant and takes no gradient")
-    if ids.dtype not in (torch.int32, torch.int64) or ids.shape not in (x.shape[:1], x.shape[:-1]):
+    if ids.dtype not in (torch.int32, torch.int64) or ids.shape not in (xs[:1], xs[:-1]):
         raise ValueError("lora_linear: adapter_ids int32, one for each sequence (x.shape[:1]) or row (x.shape[:-1])")
-    return ids if ids.dtype == torch.int32 else ids.clamp(-1, a.shape[0]).to(torch.int32)
+    return ids if ids.dtype == torch.int32 else ids.clamp(-1, fs[0]).to(torch.int32)
 
 
 def lora_linear(x, weight, lora_a, lora_b, adapter_ids, scaling):

@@ -212,8 +212,7 @@ class _SoftcapLogProbs(torch.autograd.Function):
         if g is None and h is None:
             return (None,) * 6
         logits, targets, lse, ent = ctx.saved_tensors
-        return (ops._softcap_log_probs_backward(logits.device, logits, targets, lse, ent, ops._c(g), ops._c(h), *ctx.args,
-                                                None), *(None,) * 5)
+        return (ops.softcap_log_probs_backward(logits, targets, lse, ent, ops._c(g), ops._c(h), *ctx.args), *(None,) * 5)
 
 
 class _PolicyLoss(torch.autograd.Function):
@@ -238,7 +237,7 @@ class _PolicyLoss(torch.autograd.Function):
         if grad is None:
             return (None,) * 13
         logits, targets, lse, slope = ctx.saved_tensors
-        return (ops._softcap_log_probs_backward(logits.device, logits, targets, lse, None, slope, None, *ctx.args, grad),
+        return (ops.softcap_log_probs_backward(logits, targets, lse, None, slope, None, *ctx.args, grad),
                 *(None,) * 12)
 
 
@@ -295,7 +294,7 @@ class _PreferenceLoss(torch.autograd.Function):
         if grad is None:
             return (None,) * 13
         logits, targets, lse, slope = ctx.saved_tensors
-        return (ops._softcap_log_probs_backward(logits.device, logits, targets, lse, None, slope, None, *ctx.args, grad),
+        return (ops.softcap_log_probs_backward(logits, targets, lse, None, slope, None, *ctx.args, grad),
                 *(None,) * 12)
 
 
@@ -375,14 +374,14 @@ def policy_loss(logits, targets, old_log_probs, advantages, vocab, softcap=15.0,
         raise ValueError("policy_loss: clip must be in [0, 1] and clip_high not negative")
     lo, hi = 1.0 - clip, 1.0 + clip_high
     if logits.is_cuda and logits.dtype == torch.bfloat16:
-        if w is not None:  # rows of weight 0 need not be read
-            t = torch.where(w != 0, t, ignore_index)
         grad = torch.is_grad_enabled() and logits.requires_grad
-        args = (flat, t, old, adv, ref, w, vocab, float(softcap), ignore_index, lo, hi, float(kl_coef))
+        args = old, adv, ref, w, vocab, float(softcap), ignore_index, lo, hi, float(kl_coef)
         if grad and expected_grad and flat.shape[0] and ops.policy_fused_supported(flat.shape[1]):
-            loss, logp, stats = _PolicyLossFused.apply(*args, float(expected_grad))
+            loss, logp, stats = _PolicyLossFused.apply(flat, t, *args, float(expected_grad))
         else:
-            loss, logp, stats = _PolicyLoss.apply(*args, grad)
+            if w is not None:  # rows of weight 0 are not read
+                t = torch.where(w != 0, t, ignore_index)
+            loss, logp, stats = _PolicyLoss.apply(flat, t, *args, grad)
         return PolicyLoss(loss, logp if targets.ndim == 1 else logp.view(targets.shape), *stats.unbind(0))
     if w is not None:
         t = torch.where(w != 0, t, ignore_index)

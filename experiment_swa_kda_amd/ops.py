@@ -895,8 +895,7 @@ def lora_backward(x, w16, a, b, ids, scale, u, grad, need_x, need_a, need_b):
 
 
 def _lora_backward(dev, per, x, w16, a, b, ids, scale, u, grad, need_x, need_a, need_b):
-    """lora_backward on checked and contiguous operands (on autograd's thread, which wakes up for it, a
-    check costs twice what it does elsewhere)."""
+    """lora_backward on checked and contiguous operands (as softcap_log_probs_backward's)."""
     (M, K), N, (n, R) = x.shape, w16.shape[0], a.shape[:2]
     lib = _lib.load()
     how = _lora_way(M, N, K)
@@ -967,21 +966,12 @@ def softcap_log_probs_forward(logits, targets, vocab, softcap, ignore_index=-1, 
     return (logp, lse, ent, logp64) if double else (logp, lse, ent)
 
 
-def softcap_log_probs_backward(logits, targets, lse, entropy, g, h, vocab, softcap, ignore_index=-1, *, scale=None):
+def softcap_log_probs_backward(logits, targets, lse, entropy, g, h, vocab, softcap, ignore_index=-1, scale=None):
     """Logit gradient [rows, stride] bf16 for row gradients ``g`` of the log-probabilities and ``h``
-    of the entropies (f32 [rows], either None), both times the one-element tensor ``scale``."""
-    what = "softcap_log_probs_backward"
-    dev = _token_inputs(what, logits, targets, lse, entropy, g, h)
-    if g is None and h is None or h is not None and entropy is None:
-        raise RuntimeError(f"{what}: a row gradient is needed, and for the entropies' the entropies")
-    logits, targets, lse, entropy, g, h = (_c(t) for t in (logits, targets, lse, entropy, g, h))
-    if scale is not None:
-        scale = scale.to(device=dev, dtype=torch.float32).reshape(1).contiguous()
-    return _softcap_log_probs_backward(dev, logits, targets, lse, entropy, g, h, vocab, softcap, ignore_index, scale)
-
-
-def _softcap_log_probs_backward(dev, logits, targets, lse, entropy, g, h, vocab, softcap, ignore_index, scale):
-    """softcap_log_probs_backward on checked and contiguous operands."""
+    of the entropies (f32 [rows], either None), both times the f32 scalar tensor ``scale``.  The operands
+    are the forward's, checked there, and contiguous: on autograd's thread, which wakes up for it, a
+    check costs twice what it does elsewhere."""
+    dev = logits.device
     rows, stride = logits.shape
     grad = torch.empty_like(logits)
     with _on(dev):

@@ -344,6 +344,35 @@ def test_two_captured_losses_take_turns(cols):
             assert all(torch.equal(a, b) for a, b in zip(o, w)), turn
 
 
+@pytest.mark.parametrize("cols", [1024, 40000])
+def test_policy_rows_of_weight_zero_are_not_read(cols):
+    """In every form of the loss, NaN logits, advantages and old values of such rows reach nothing."""
+    x, t, (old, adv, ref, w) = case(9, 1000, cols, 16, ignore_every=0)
+    w = w.abs() + 0.1
+    off = torch.tensor([0, 4, 8])
+    w[off] = 0.0
+    clean = [v.clone() for v in (x, old, adv, ref)]
+    for v in (x, old, adv, ref):
+        v[off] = float("nan")
+    got, grads = [], []
+    for values, expected in ((clean, 1.0), ((x, old, adv, ref), 1.0), ((x, old, adv, ref), None), ((x, old, adv, ref), 0.5)):
+        leaf = values[0].cuda().requires_grad_()
+        r = policy_loss(leaf, t.cuda(), values[1].cuda(), values[2].cuda(), 1000, ref_log_probs=values[3].cuda(), clip=1.0,
+                        clip_high=9.0, kl_coef=0.1, weights=w.cuda(), expected_grad=expected)
+        got.append(r)
+        grads.append(torch.autograd.grad(r.loss, leaf)[0])
+        with torch.no_grad():
+            got.append(policy_loss(leaf, t.cuda(), values[1].cuda(), values[2].cuda(), 1000, ref_log_probs=values[3].cuda(),
+                                   clip=1.0, clip_high=9.0, kl_coef=0.1, weights=w.cuda()))
+    for r in got:
+        assert not r.log_probs[off].any() and torch.isfinite(r.log_probs).all()
+        # the same f64 terms, from sums of e^z in one order or another (EPS) and slopes of some e^9
+        assert abs(r.loss.item() - got[0].loss.item()) <= 20 * eps_of(1000) * max(1.0, abs(got[0].loss.item()))
+    for g in grads:
+        assert not g[off].any() and torch.isfinite(g).all()
+    assert torch.equal(grads[0], grads[1])
+
+
 def test_entropy_gradient_of_a_target_outside_the_vocabulary():
     """Its log-probability is NaN; the row's entropy and the entropy's gradient are the row's own."""
     x, t, (_, _, _, h) = case(6, 1000, 1024, 14, ignore_every=0)
