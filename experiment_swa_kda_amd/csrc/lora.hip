@@ -21,7 +21,7 @@ namespace kda {
 // shrink: one workgroup per 16 MT rows; its waves take 64 columns of J at a time each, and their
 // partial tiles meet in LDS.  RT = ceil(R / 16).  Lanes load along rows (8 lanes to a 128-byte line:
 // an MFMA fragment loaded directly has 16 rows in 16 neighbouring lanes, 64 cycles of address
-// processing for its 1 KB instead of 16: 7777 x 4096 at rank 64 took 48 us, now 12, 5.2 TB/s) and pass the rows
+// processing for its 1 KB instead of 16: 7777 x 4096 at rank 64 took 48 us, now 22, 2.9 TB/s) and pass the rows
 // through an LDS stage of their own, so without a barrier; AHEAD groups of 64 columns are in flight.
 // TRANSPOSED: F is [n, J, R], its fragments run down the stage's columns.
 // ---------------------------------------------------------------------------------------
@@ -176,8 +176,8 @@ __global__ __launch_bounds__(kShrinkWaves * kWave) void lora_shrink_kernel(LoraR
 // expand: 64 rows x 256 columns per workgroup; wave w has rows 16 w .. and keeps their u in
 // registers.  KS = ceil(R / 32) steps of the contraction.  F passes through LDS in pieces of 64
 // columns, the next piece on its way; so does the result, to be stored along rows.  TRANSPOSED: F is
-// [n, R, J].  Bound by the write of y: 7777 x 2048 and x 4096 at rank 64 take 13 and 18 us (2.4 and 3.5
-// TB/s), 8192 x 32768 at rank 16 156 us (3.4).
+// [n, R, J].  Bound by the write of y: 7777 x 2048 and x 4096 at rank 64 take 15 and 23 us (2.1 and 2.8
+// TB/s), 8192 x 32768 at rank 16 159 us (3.4).
 // ---------------------------------------------------------------------------------------
 constexpr int kExpandCols = 256;
 
@@ -317,8 +317,9 @@ __global__ __launch_bounds__(256) void lora_expand_rows_kernel(LoraRows rows, in
 // that hold a row of the adapter, with the other rows masked and the next step's loads in flight, and
 // leaves an f32 partial and a flag; a second kernel sums the flagged partials in order.  A single
 // range is the result itself (flag null).  COLS: the result is [n, J, R], else [n, R, J].
-// Bound by reading x once and u once for every 128 columns: 8192 x 32768 at rank 16 takes 122 us with
-// the sum (4.4 TB/s), 7777 x 4096 at rank 64, three adapters, 36 + 6 (the ranges' partials are 18 MB).
+// Bound by reading x once and u's three parts for every 128 columns: 8192 x 32768 at rank 16 takes 128 us
+// with the sum (4.2 TB/s of x), 7777 x 4096 at rank 64 45 us (1.4: there u's parts are more than x, and the
+// ranges' partials 22 MB).
 // ---------------------------------------------------------------------------------------
 constexpr int kGradCols = 128;
 constexpr int kGradRows = 64;
@@ -515,9 +516,10 @@ extern "C" int kda_lora_shrink(int64_t M, int32_t J, int32_t R, int32_t n, const
     hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(kShrinkWaves * kWave), 0, stream, rows, seq_tiles, J, R,
                        (const bf16*)x, (long)ldx, (const bf16*)factor, scale, (bf16*)u);
   };
-  // 32 rows share a read of the factor where that leaves work for every CU: 65536 x 4096 at rank 128 takes
-  // 225 us against 332 in tiles of 16, 8192 x 1536 at rank 16 5.7 / 6.3, but 4096 x 4096 at rank 64 16.3 / 13.0
-  auto pick = [&](auto k1, auto k2) { M >= 8192 ? go(k2, 2) : go(k1, 1); };
+  // 32 rows share a read of the factor where there are more than 16 for every CU (x from memory, us, tiles of
+  // 32 / 16: 6144 x 4096 at rank 64 20 / 26, 8192 x 4096 at rank 128 31 / 44, 8192 x 1536 at rank 16 8.3 / 8.6, but
+  // 4096 x 4096 at rank 64 19 / 15)
+  auto pick = [&](auto k1, auto k2) { M > 4096 ? go(k2, 2) : go(k1, 1); };
   if (factor_cols) {
     if (R <= 16) pick(lora_shrink_kernel<1, 1, true>, lora_shrink_kernel<1, 2, true>);
     else if (R <= 32) pick(lora_shrink_kernel<2, 1, true>, lora_shrink_kernel<2, 2, true>);
