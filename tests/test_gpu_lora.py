@@ -240,6 +240,17 @@ def test_empty_and_single():
     check({**d, "x": d["x"][:, :1]} | {"dy": d["dy"][:, :1]}, torch.tensor([1, 0]), two)
 
 
+def test_second_derivatives_are_refused():
+    d, ids, _ = case(3, 30, 64, 96, 16, 2, 18, masters=True)
+    leaves = [d[k].detach().requires_grad_() for k in ("x", "a", "b")]
+    y = lora_linear(leaves[0], d["w"], *leaves[1:], ids.cuda(), d["scale"])
+    first = torch.autograd.grad(y, leaves, d["dy"], retain_graph=True)
+    again = torch.autograd.grad(y, leaves, d["dy"], create_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(first, again))
+    with pytest.raises(RuntimeError, match="once_differentiable|does not require grad"):
+        torch.autograd.grad(again[1].sum(), leaves[2])
+
+
 def test_gpu_refusals():
     d, ids, _ = case(2, 3, 64, 96, 16, 2, 8)
     cuda = ids.cuda()

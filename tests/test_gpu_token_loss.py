@@ -386,6 +386,22 @@ def test_entropy_gradient_of_a_target_outside_the_vocabulary():
     check_grad(grad, x, inside, 1000, np.zeros(6), n(h))
 
 
+@pytest.mark.parametrize("expected", [1.0, None])
+def test_second_derivatives_are_refused(expected):
+    """create_graph gives the same first gradient; differentiating it again is an error, not zero."""
+    x, t, (old, adv, ref, _) = case(8, 1000, 1024, 17)
+    leaf = x.cuda().requires_grad_()
+    calls = [lambda: softcap_log_probs(leaf, t.cuda(), 1000).sum(),
+             lambda: policy_loss(leaf, t.cuda(), old.cuda() - 8, adv.cuda(), 1000, expected_grad=expected).loss,
+             lambda: preference_loss(leaf.view(4, 2, -1), t.cuda().view(4, 2), 1000).loss]
+    for call in calls:
+        (first,) = torch.autograd.grad(call(), leaf)
+        (again,) = torch.autograd.grad(call(), leaf, create_graph=True)
+        assert torch.equal(first, again)
+        with pytest.raises(RuntimeError, match="once_differentiable|does not require grad"):
+            torch.autograd.grad(again.float().square().sum(), leaf)
+
+
 def test_offsets_past_32_bits():
     """70000 rows of 32768 columns, 2.3e9 logits, with a few counted rows at both ends."""
     rows, vocab = 70000, 32768
