@@ -1018,7 +1018,9 @@ class KimiDeltaAttention(nn.Module):
             return False
         # (by name from the dicts: attribute access of a module costs a microsecond each)
         linears, convs = [self._modules[n] for n in _LINEARS], [self._modules[n] for n in _CONVS]
-        if any([type(m) is not Linear or m._parameters["bias"] is not None for m in linears]) or any(
+        # (the output projection, last, is called as a module: with adapters too)
+        if any([(type(m) is not Linear and (m is not linears[-1] or type(m) is not LoraLinear))
+                or m._parameters["bias"] is not None for m in linears]) or any(
                 [type(m) is not ShortConvolution or m.kernel_size != (4,) for m in convs]) or not plain(*linears, *convs):
             return False
         weights = [m._parameters.get("weight") for m in (*linears, *convs)]

@@ -683,7 +683,7 @@ class Block(nn.Module):
         fc, proj = mlp._modules["c_fc"], mlp._modules["c_proj"]
         if not attn.mode.startswith("project_") or attn._cached16() is None or not plain(attn, mlp, fc, proj):
             return False
-        if type(fc) is not Linear or type(proj) is not Linear or fc.bias is not None or proj.bias is not None:
+        if any([type(m) is not Linear or m._parameters["bias"] is not None for m in (fc, proj, attn._modules["o_proj"])]):
             return False
         w1, w2 = getattr(fc, "_w16", None), getattr(proj, "_w16", None)
         if w1 is None or w2 is None or w1.shape[0] % 32 or w2.shape != (x.shape[-1], w1.shape[0]):

@@ -20,7 +20,7 @@ pytestmark = pytest.mark.gpu
 if torch.cuda.is_available():
     from experiment_swa_kda_amd import KimiDeltaAttention, lora_linear, ops
     from experiment_swa_kda_amd.kda import Linear, LoraLinear
-    from experiment_swa_kda_amd.model import GPT, GPTConfig, GraphedUpdate, KVCache
+    from experiment_swa_kda_amd.model import GPT, Block, GPTConfig, GraphedUpdate, KVCache
 
 
 def n64(t):
@@ -376,6 +376,62 @@ def test_decoder_serves_a_batch_of_requests_with_their_own_adapters():
         # as two bf16 forwards of 2 layers and a head are (logits of a few units)
         assert (alone[0] - mixed[row]).abs().max().item() < 0.25
         assert (alone[0] - mixed[row]).norm() < 0.03 * alone[0].norm()
+
+
+def test_adapters_of_the_output_projection_alone_are_not_passed_over():
+    """A block whose MLP is plain: its one-token step still adds the output projection's adapters."""
+    m = small_gpt(4)
+    for b in m.transformer.h:
+        lin = LoraLinear(128, 128, 2, 8).cuda()
+        lin.weight = b.attn.o_proj.weight
+        torch.nn.init.normal_(lin.lora_b, 0.0, 0.1)
+        b.attn.o_proj = lin
+    ids = torch.tensor([1, -1, 0], dtype=torch.int32, device="cuda")
+    idx = torch.randint(0, 500, (3, 12), device="cuda")
+
+    def generate(adapters):
+        m.use_adapters(adapters)
+        cache = KVCache(3, 2, 64, 64, 2, "cuda", torch.bfloat16)
+        m.cache_bf16_weights()
+        with torch.no_grad():
+            out = [m(idx[:, :8], kv_cache=cache)[:, -1]] + [m(idx[:, k:k + 1], kv_cache=cache)[:, -1] for k in range(8, 12)]
+        m.drop_bf16_weights()
+        return torch.stack(out, 1)
+
+    got, bare = generate(ids), generate(None)
+    m.use_adapters(ids)
+    with torch.no_grad():
+        full = m(idx)[:, 7:]  # the whole sequence at once: no state, no token step
+    # a step's activations and the prompt's are bf16 roundings of the same values, two layers of them
+    assert (got - full).norm() <= 0.03 * full.norm()
+    # without the one-token step that computes with a plain projection's weight: the same kernels, bit for bit
+    kept = Block._token_ok
+    try:
+        Block._token_ok = lambda *args: False
+        assert torch.equal(generate(ids), got)
+    finally:
+        Block._token_ok = kept
+    # (a row's computation does not depend on the other rows: what differs from the bare model is the adapters')
+    same = (got == bare).flatten(1).all(1).tolist()
+    assert same == [False, True, False]
+
+
+def test_adapter_gradients_beside_frozen_weights():
+    """With the weights frozen the mixers' cores below run outside autograd: the adapters' gradients are
+    those of the model that trains everything."""
+    m = small_gpt(5)
+    new = m.add_adapters(2, 8)
+    with torch.no_grad():
+        for p in new:
+            p.normal_(0.0, 0.05)
+    m.use_adapters(torch.tensor([1, 0], dtype=torch.int32, device="cuda"))
+    idx = torch.randint(0, 500, (2, 40), device="cuda")
+    want = torch.autograd.grad(m(idx[:, :-1], idx[:, 1:]), new)
+    for p in m.parameters():
+        p.requires_grad_(any(p is q for q in new))
+    got = torch.autograd.grad(m(idx[:, :-1], idx[:, 1:]), new)
+    for p, q in zip(got, want):
+        assert q.any() and (p - q).norm() <= 0.02 * q.norm()  # (the same chain of bf16 roundings, 2^-8 each)
 
 
 def test_decoder_trains_adapters_on_the_policy_loss():
