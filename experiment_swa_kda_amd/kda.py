@@ -259,7 +259,7 @@ def _cast16(*tensors):
     if all(t.is_cuda and t.dtype == torch.float32 and t.is_contiguous() and t.numel() % 8 == 0 and t.numel() and t.data_ptr() % 16 == 0
            and t.device == tensors[0].device for t in tensors):
         counts = [t.numel() for t in tensors]
-        parts = torch.split(ops.cast_weights_bf16([t.detach() for t in tensors], counts), counts)
+        parts = torch.split(ops.cast_weights_bf16(tensors, counts), counts)
         return [p.view(t.shape) for p, t in zip(parts, tensors)]
     return [t if t.dtype == torch.bfloat16 else t.detach().to(torch.bfloat16) for t in tensors]
 
